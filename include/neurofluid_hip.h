@@ -580,6 +580,44 @@ int nf_trans_step(const nf_trans_step_t* s /*[host]*/, const float* pos, const f
                   float* vel_c, int32_t* host_flag3 /* as nf_trans_front's; inside the step [2] = step_id is raised by the first layer's launch as it
                                                        starts (the searches and their overflow words [0], [1] are complete then) */, int step_id, nf_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Gated linear recurrence over sequences, beside the compositing kernels: nf_composite_fwd / _bwd (models/renderer.py:182-208) are
+ * this recurrence for three channels, run towards the eye with the gate 1 - alpha; here the channels, the gates and the
+ * direction are the caller's.
+ *     h_t = A_t h_{t-1} + x_t,   A_t = gate_t, or exp(gate_t) when log_gate (-sigma delta of a ray's sample, a decay)
+ * nf_scan_fwd writes every state (h, the storage type) and the final ones (h_last, fp32); nf_scan_bwd the gradients
+ *     dx_t = g_t + u_{t+1},  u_t = A_t dx_t,  dgate_t = dx_t h_{t-1} (log_gate: u_t h_{t-1}; shared: summed over the channels),  dh0 = u_first
+ * with u behind the last step = g_last.  States, products and sums are fp32; what is stored in 16 bits is rounded once, to nearest.
+ * The stretch products carry states over long distances: gates are meant to be decays (|A| <= 1), larger ones overflow there sooner than
+ * step by step.  Results repeat bit for bit.
+ * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, nw; *state_floats = the size
+ * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_floats =
+ * nf_scan_workspace_floats(s, backward) floats.  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
+ * h0, states (and sid).
+ * row_splits (device, n_seq + 1, ascending): B = 1 and the T rows hold n_seq sequences behind one another, h0 / h_last / g_last / dh0 have
+ * one row for each (an empty sequence passes them through); h, dx, dgate are zero on rows that belong to none.  sid: T ints, filled by the
+ * forward.  dense with T = 0: nothing is written. */
+typedef struct {
+    int dtype /*0 fp32, 1 bf16, 2 fp16: x, h, g, dx*/, gate32 /*gate, dgate in fp32*/, shared /*one gate a step*/, log_gate, reverse;
+    int B, T, D, n_seq;
+    const int64_t* row_splits /*or NULL*/;
+    const void* gate; const void* x; const void* g /*or NULL*/;
+    const float* h0 /*(B or n_seq, D) or NULL*/; const float* g_last /*or NULL*/;
+    int64_t gate_sb, gate_st, x_sb, x_st, g_sb, g_st;
+    void* h; float* h_last; float* states /*forward: or NULL*/; int32_t* sid /*packed*/;
+    void* dgate /*or NULL*/; void* dx /*or NULL*/; float* dh0 /*or NULL*/;
+    int vec, cg, nw;
+    float* workspace; size_t workspace_floats;
+} nf_scan_t;
+int nf_scan_plan(nf_scan_t* s /*[host]*/, size_t* state_floats /*[host]*/);
+size_t nf_scan_workspace_floats(const nf_scan_t* s /*[host]*/, int backward);
+int nf_scan_fwd(const nf_scan_t* s /*[host]*/, nf_stream_t stream);
+int nf_scan_bwd(const nf_scan_t* s /*[host]*/, nf_stream_t stream);
+/* One step for `rows` independent states: next = A state + x (fp32, row strides in elements; next may be state itself), h = next in
+ * the storage type (contiguous). */
+int nf_scan_step(int dtype, int gate32, int shared, int log_gate, int rows, int D, const void* gate, int64_t gate_stride, const void* x,
+                 int64_t x_stride, const float* state, int64_t state_stride, float* next, int64_t next_stride, void* h, nf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,15 @@ class TransStep(ctypes.Structure):
                [(k, c_float) for k in ("radius", "extent", "dt", "scale")] + [("gravity", c_float * 3), ("bbox", c_float * 6), ("split", c_int), ("search", c_int)]
 
 
+class Scan(ctypes.Structure):
+    """nf_scan_t (include/neurofluid_hip.h)."""
+    _fields_ = [(k, c_int) for k in ("dtype", "gate32", "shared", "log_gate", "reverse", "B", "T", "D", "n_seq")] + \
+               [(k, c_void_p) for k in ("row_splits", "gate", "x", "g", "h0", "g_last")] + \
+               [(k, c_int64) for k in ("gate_sb", "gate_st", "x_sb", "x_st", "g_sb", "g_st")] + \
+               [(k, c_void_p) for k in ("h", "h_last", "states", "sid", "dgate", "dx", "dh0")] + \
+               [(k, c_int) for k in ("vec", "cg", "nw")] + [("workspace", c_void_p), ("workspace_floats", c_size_t)]
+
+
 # name -> (restype, argtypes); mirrors include/neurofluid_hip.h one-to-one (tests check the list)
 PROTOTYPES = {
     "nf_version": (c_int, []),
@@ -163,6 +172,12 @@ PROTOTYPES = {
     "nf_gather_view_pixels_tab": (c_int, [c_int, c_void_p, c_int, c_int, ctypes.c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nf_e2e_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, ctypes.POINTER(c_float), ctypes.POINTER(c_float), c_float,
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nf_scan_plan": (c_int, [ctypes.POINTER(Scan), ctypes.POINTER(c_size_t)]),
+    "nf_scan_workspace_floats": (c_size_t, [ctypes.POINTER(Scan), c_int]),
+    "nf_scan_fwd": (c_int, [ctypes.POINTER(Scan), c_void_p]),
+    "nf_scan_bwd": (c_int, [ctypes.POINTER(Scan), c_void_p]),
+    "nf_scan_step": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                             c_void_p, c_void_p]),
     "nf_trans_step": (c_int, [ctypes.POINTER(TransStep), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                               c_void_p]),
 }

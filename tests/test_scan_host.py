@@ -1,0 +1,74 @@
+"""The gated recurrence's refusals: everything that is refused is refused on the host, before anything touches a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from neurofluid_amd import scan
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("gate, x, kw, err", [
+    (t(2, 5, 3, dtype=torch.float64), t(2, 5, 3, dtype=torch.float64), {}, TypeError),
+    (t(2, 5, 3, dtype=torch.bfloat16), t(2, 5, 3), {}, TypeError),                       # a 16-bit gate beside 32-bit x
+    (t(2, 5, 3, dtype=torch.float16), t(2, 5, 3, dtype=torch.bfloat16), {}, TypeError),
+    (t(2, 5, 2), t(2, 5, 3), {}, ValueError),
+    (t(1, 5, 3), t(2, 5, 3), {}, ValueError),                                             # (expand() it)
+    (t(5, 3), t(2, 5, 3), {}, ValueError),
+    (t(2, 5, 0), t(2, 5, 0), {}, ValueError),
+    (t(5, 3), t(5, 3), {}, ValueError),                                                   # 2-d without row_splits
+    (t(2, 5, 3), t(2, 5, 3), dict(row_splits=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (t(5, 3), t(5, 3), dict(row_splits=torch.zeros(2, dtype=torch.int32)), ValueError),
+    (t(5, 3), t(5, 3), dict(row_splits=torch.zeros(0, dtype=torch.int64)), ValueError),
+    (t(5, 3), t(5, 3), dict(row_splits=torch.zeros(3, dtype=torch.int64), h0=t(3, 3)), ValueError),
+    (t(2, 5, 3), t(2, 5, 3), dict(h0=t(2, 4)), ValueError),
+    (t(2, 5, 3), t(2, 5, 3), dict(h0=t(2, 3, dtype=torch.bfloat16)), ValueError),
+    (t(2, 5, 3), t(2, 5, 3), {}, RuntimeError),                                           # on the CPU: no fallback
+])
+def test_gated_scan_refuses(gate, x, kw, err):
+    with pytest.raises(err):
+        scan.gated_scan(gate, x, **kw)
+
+
+@pytest.mark.parametrize("gate, x, state, kw, err", [
+    (t(2, 5, 3), t(2, 5, 3), t(2, 5, 3), {}, ValueError),
+    (t(4, 3), t(4, 3), t(4, 2), {}, ValueError),
+    (t(4, 3), t(4, 3), t(4, 3, dtype=torch.float16), {}, ValueError),
+    (t(4, 3), t(4, 3), t(3, 4).t(), {}, ValueError),                                      # channels apart
+    (t(4, 3), t(4, 3), t(1, 3).expand(4, 3), {}, ValueError),                             # one state for all rows
+    (t(4, 3), t(4, 3), t(4, 3), dict(out=t(4, 1).expand(4, 3)), ValueError),
+    (t(4, 3).requires_grad_(), t(4, 3), t(4, 3), {}, RuntimeError),
+    (t(4, 3), t(4, 3), t(4, 3), {}, RuntimeError),
+])
+def test_gated_scan_step_refuses(gate, x, state, kw, err):
+    with pytest.raises(err):
+        scan.gated_scan_step(gate, x, state, **kw)
+
+
+def test_gated_scan_step_refuses_an_out_that_overlaps_the_state():
+    buf = t(6, 3)
+    with pytest.raises(ValueError, match="overlaps"):
+        scan.gated_scan_step(t(4, 3), t(4, 3), buf[:4], out=buf[1:5])
+
+
+def test_c_entries_refuse():
+    from neurofluid_amd import _lib, build
+    build.build()
+    lib = _lib.load()
+    s = _lib.Scan(dtype=7, B=1, T=4, D=4)
+    assert lib.nf_scan_plan(ctypes.byref(s), None) < 0 and b"dtype" in lib.nf_last_error()
+    s = _lib.Scan(dtype=0, B=1, T=4, D=0)
+    assert lib.nf_scan_plan(ctypes.byref(s), None) < 0 and b"sizes" in lib.nf_last_error()
+    s = _lib.Scan(dtype=0, B=1, T=4, D=4)
+    assert lib.nf_scan_fwd(ctypes.byref(s), None) < 0 and b"plan" in lib.nf_last_error()
+    n = ctypes.c_size_t()
+    assert lib.nf_scan_plan(ctypes.byref(s), ctypes.byref(n)) == 0 and s.vec in (1, 2) and n.value >= 4
+    assert lib.nf_scan_fwd(ctypes.byref(s), None) < 0 and b"null" in lib.nf_last_error()
+    assert lib.nf_scan_step(0, 0, 0, 0, -1, 4, None, 0, None, 0, None, 0, None, 0, None, None) < 0
+    assert lib.nf_scan_step(0, 0, 0, 0, 1, 4, None, 0, None, 0, None, 0, None, 0, None, None) < 0
+    # a long, narrow sequence is cut: the plan asks for room for the chunks
+    s = _lib.Scan(dtype=1, B=1, T=100000, D=64)
+    assert lib.nf_scan_plan(ctypes.byref(s), None) == 0 and lib.nf_scan_workspace_floats(ctypes.byref(s), 0) > 0
