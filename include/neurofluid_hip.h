@@ -618,6 +618,30 @@ int nf_scan_bwd(const nf_scan_t* s /*[host]*/, nf_stream_t stream);
 int nf_scan_step(int dtype, int gate32, int shared, int log_gate, int rows, int D, const void* gate, int64_t gate_stride, const void* x,
                  int64_t x_stride, const float* state, int64_t state_stride, float* next, int64_t next_stride, void* h, nf_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Activations kept in 8 bits between forward and backward, beside nf_nerf_wgrad / nf_gemm_f32 (what torch autograd keeps for the
+ * nn.Linear layers of models/nerf.py:55-81 in 32 bits).
+ * Form of an (rows, K) matrix: e4m3 codes, rows of 32 ceil(K / 32) bytes (zeros behind K), and for every 32 features of a row one scale 2^k, the
+ * smallest power of two that brings the largest finite magnitude to 448 or less, k >= -110; scales hold k + 127, block by block:
+ * [ceil(K / 32)][64 ceil(rows / 64)] bytes.  code = x / 2^k to nearest even, magnitudes above 1.875 2^127
+ * taken as that; a value that is not finite becomes NaN.  A value is off by at most
+ * 2^-4 of itself, or 2^(k - 10) where that is more.  dtype: 0 fp32, 1 bf16, 2 fp16; strides in elements, features adjacent.  Unpacked fp16 rounds
+ * (and overflows) where fp16 does not hold the value. */
+size_t nf_act8_code_bytes(int rows, int K);
+size_t nf_act8_scale_bytes(int rows, int K);
+int nf_act8_pack(int dtype, const void* x, int64_t x_stride, int rows, int K, uint8_t* codes, uint8_t* scales, nf_stream_t stream);
+int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* scales, int rows, int K, void* out, int64_t out_stride, nf_stream_t stream);
+/* Weight and bias gradients of up to 16 linear layers that read one packed matrix, in one launch and the slices' reduction:
+ *     dW_j[m][k] = sum_r dy[r][dy_col_j + m] x^[r][x_col_j + k],     db_j[m] = sum_r dy[r][dy_col_j + m]    (bias_j != 0)
+ * x^ = the values the codes stand for.  fp32 results: every product is exact (but for what of dy lies below 2^-133), sums are
+ * fp32 in a fixed order.  dweights holds the dW_j [M][K] one
+ * behind the other, dbias the db_j of the jobs that ask for one.  x_col_j must be a multiple of 32.  rows = 0 gives zeros.
+ * workspace: nf_act8_wgrad_workspace_floats floats. */
+typedef struct { int dy_col, M, x_col, K, bias; } nf_act8_job_t;
+size_t nf_act8_wgrad_workspace_floats(int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs /*[host]*/);
+int nf_act8_wgrad(int dtype, const void* dy, int64_t dy_stride, int dy_cols, const uint8_t* codes, const uint8_t* scales, int x_cols, int rows,
+                  int njobs, const nf_act8_job_t* jobs /*[host]*/, float* workspace, float* dweights, float* dbias, nf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,11 @@ class Scan(ctypes.Structure):
                [(k, c_int) for k in ("vec", "cg", "nw")] + [("workspace", c_void_p), ("workspace_floats", c_size_t)]
 
 
+class Act8Job(ctypes.Structure):
+    """nf_act8_job_t (include/neurofluid_hip.h)."""
+    _fields_ = [(k, c_int) for k in ("dy_col", "M", "x_col", "K", "bias")]
+
+
 # name -> (restype, argtypes); mirrors include/neurofluid_hip.h one-to-one (tests check the list)
 PROTOTYPES = {
     "nf_version": (c_int, []),
@@ -178,6 +183,13 @@ PROTOTYPES = {
     "nf_scan_bwd": (c_int, [ctypes.POINTER(Scan), c_void_p]),
     "nf_scan_step": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                              c_void_p, c_void_p]),
+    "nf_act8_code_bytes": (c_size_t, [c_int, c_int]),
+    "nf_act8_scale_bytes": (c_size_t, [c_int, c_int]),
+    "nf_act8_pack": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "nf_act8_unpack": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p]),
+    "nf_act8_wgrad_workspace_floats": (c_size_t, [c_int, c_int, c_int, c_int, ctypes.POINTER(Act8Job)]),
+    "nf_act8_wgrad": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, ctypes.POINTER(Act8Job), c_void_p, c_void_p,
+                              c_void_p, c_void_p]),
     "nf_trans_step": (c_int, [ctypes.POINTER(TransStep), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                               c_void_p]),
 }

@@ -1,0 +1,176 @@
+"""Activations kept in 8 bits between forward and backward (csrc/nf_act8.hip), and the weight gradients that read them.
+
+What torch autograd keeps for the linear layers of models/nerf.py:55-81 are their inputs, in 32 bits.  ``pack`` keeps them as e4m3 codes with one
+power-of-two scale for every 32 features of a row (1.03 bytes a value, off by at most 2^-4 of itself), ``wgrad`` computes dW = dy^T x^ and
+db = sum dy from the codes as they are, ``linear`` is the layer that does both, and ``NeRF(..., act_checkpoint="e4m3")`` trains on it.
+Forward values and the gradients of the inputs are those of the exact activations; only the weights' gradients see the 8 bits.
+There is no torch fallback: CPU tensors raise.
+"""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from ._lib import check, ptr
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MAX = 1 << 30
+
+
+def _matrix(t):
+    """t's last axis as columns, everything before as rows; columns adjacent (a copy where the layout asks for one)."""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return m if m.shape[1] <= 1 or m.stride(1) == 1 else m.contiguous()
+
+
+class Act8:
+    """A matrix in 8 bits: ``codes`` and ``scales`` (uint8, the layout of nf_act8_pack), ``shape`` and ``dtype`` of what was packed."""
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
+
+    @property
+    def features(self):
+        return self.shape[-1]
+
+    @property
+    def rows(self):
+        n = 1
+        for k in self.shape[:-1]:
+            n *= k
+        return n
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def unpack(self, dtype=None):
+        """The values that the codes stand for, in ``dtype`` (default: what was packed)."""
+        dtype = dtype or self.dtype
+        if dtype not in _DTYPES:
+            raise TypeError(f"Act8.unpack: float32, bfloat16 or float16, not {dtype}")
+        lib = _lib.load()
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            check(lib.nf_act8_unpack(_DTYPES[dtype], ptr(self.codes), ptr(self.scales), self.rows, self.features, ptr(out), self.features, _lib.stream()),
+                  "nf_act8_unpack")
+        return out
+
+
+def pack(x):
+    """x (..., K) float32 / bfloat16 / float16 -> Act8.  The scale of a block of 32 features is the smallest power of two (2^-110 at least) that
+    brings its largest finite magnitude to 448 or less; codes are rounded to nearest even; values that are not finite become NaN."""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"act8.pack: x must be float32, bfloat16 or float16, not {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("act8.pack: x needs at least one axis")
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    if rows > _MAX or x.shape[-1] > _MAX:
+        raise ValueError(f"act8.pack: more than {_MAX} rows or features")
+    ops._require_cuda(x)
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        m = _matrix(x.detach()) if rows else x.detach()
+        codes = torch.empty(lib.nf_act8_code_bytes(rows, x.shape[-1]), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(lib.nf_act8_scale_bytes(rows, x.shape[-1]), dtype=torch.uint8, device=x.device)
+        if rows:
+            check(lib.nf_act8_pack(_DTYPES[x.dtype], ptr(m), m.stride(0), rows, x.shape[-1], ptr(codes), ptr(scales), _lib.stream()), "nf_act8_pack")
+    return Act8(codes, scales, x.shape, x.dtype)
+
+
+def wgrad_jobs(dy, ckpt, jobs):
+    """Weight gradients of up to 16 layers that read column ranges of one packed matrix, in one launch: jobs = [(first column of dy, outputs, first
+    feature (a multiple of 32), features, with bias)] -> [(dW (outputs, features), db (outputs) or None)], float32."""
+    if dy.dtype not in _DTYPES:
+        raise TypeError(f"act8.wgrad: dy must be float32, bfloat16 or float16, not {dy.dtype}")
+    if not isinstance(ckpt, Act8):
+        raise TypeError("act8.wgrad: the activations must be an Act8 (act8.pack)")
+    if dy.dim() < 1 or dy.shape[-1] < 1 or ckpt.features < 1 or dy.numel() // dy.shape[-1] != ckpt.rows:
+        raise ValueError(f"act8.wgrad: dy {tuple(dy.shape)} does not fit activations {ckpt.shape}")
+    if not 1 <= len(jobs) <= 16:
+        raise ValueError("act8.wgrad: 1 to 16 jobs")
+    ops._require_cuda(dy)
+    if dy.device != ckpt.device:
+        raise ValueError("act8.wgrad: dy and the activations are on different devices")
+    lib = _lib.load()
+    dev = dy.device
+    with torch.cuda.device(dev):
+        m = _matrix(dy.detach())
+        js = (_lib.Act8Job * len(jobs))(*[_lib.Act8Job(int(a), int(b), int(c), int(d), int(bool(e))) for a, b, c, d, e in jobs])
+        rows = ckpt.rows
+        args = (rows, dy.shape[-1], ckpt.features, len(jobs), js)
+        ws = torch.empty(lib.nf_act8_wgrad_workspace_floats(*args), dtype=torch.float32, device=dev)
+        dw = torch.empty(sum(b * d for _, b, _, d, _ in jobs), dtype=torch.float32, device=dev)
+        db = torch.empty(sum(b for _, b, _, _, e in jobs if e), dtype=torch.float32, device=dev)
+        check(lib.nf_act8_wgrad(_DTYPES[dy.dtype], ptr(m), m.stride(0), dy.shape[-1], ptr(ckpt.codes), ptr(ckpt.scales), ckpt.features, rows, len(jobs), js,
+                                ptr(ws), ptr(dw), ptr(db), _lib.stream()), "nf_act8_wgrad")
+    out, o, q = [], 0, 0
+    for _, b, _, d, e in jobs:
+        out.append((dw[o:o + b * d].view(b, d), db[q:q + b] if e else None))
+        o += b * d
+        q += b if e else 0
+    return out
+
+
+def wgrad(dy, ckpt, bias=True):
+    """dW = dy^T x^ (M, K) and db = the sum of dy's rows (M) of a linear layer whose input is kept as ``ckpt``, both float32 (db None without
+    ``bias``).  dy: (..., M) float32 / bfloat16 / float16, as many rows as were packed.  Products are exact, sums float32 in a fixed order."""
+    return wgrad_jobs(dy, ckpt, [(0, dy.shape[-1] if dy.dim() else 0, 0, ckpt.features if isinstance(ckpt, Act8) else 0, bias)])[0]
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        with torch.cuda.device(x.device):
+            m, w = _matrix(x.detach()), weight.detach()
+            y = torch.empty(m.shape[0], w.shape[0], dtype=torch.float32, device=x.device)
+            if bias is not None:
+                y.copy_(bias.detach().expand_as(y))
+            if m.shape[0]:
+                ops.gemm(m, w.t(), out=y, accumulate=bias is not None)
+            ctx.ckpt = pack(m) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(weight)
+        return y.view(x.shape[:-1] + (w.shape[0],))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (weight,) = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        with torch.cuda.device(g.device):
+            m = _matrix(g.detach())
+            if need[0]:
+                dx = torch.empty(m.shape[0], weight.shape[1], dtype=torch.float32, device=g.device)
+                if m.shape[0]:
+                    ops.gemm(m, weight.detach(), out=dx)
+                dx = dx.view(g.shape[:-1] + (weight.shape[1],))
+            if need[1]:
+                dw, db = wgrad(m, ctx.ckpt, bias=need[2])
+            elif need[2]:
+                db = m.sum(0)
+        return dx, dw, db
+
+
+def linear(x, weight, bias=None):
+    """torch.nn.functional.linear on float32 whose input is kept in 8 bits for the backward (4.1 times fewer bytes): y = x W^T + b and dx = dy W run
+    on the fp32 matrix pipe (ops.gemm), dW and db are ``wgrad`` of the packed input.  Differentiable once."""
+    for t, name, dims in ((x, "x", None), (weight, "weight", 2), (bias, "bias", 1)):
+        if t is None:
+            continue
+        if t.dtype != torch.float32:
+            raise TypeError(f"act8.linear: {name} must be float32, not {t.dtype}")
+        if dims is not None and t.dim() != dims:
+            raise ValueError(f"act8.linear: {name} must have {dims} axes, got {tuple(t.shape)}")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.numel() == 0 or (bias is not None and bias.shape[0] != weight.shape[0]):
+        raise ValueError(f"act8.linear: x {tuple(x.shape)}, weight {tuple(weight.shape)}"
+                         + (f", bias {tuple(bias.shape)}" if bias is not None else "") + " do not fit")
+    if any(t is not None and t.device != x.device for t in (weight, bias)):
+        raise ValueError("act8.linear: x, weight and bias are on different devices")
+    ops._require_cuda(x)
+    return _LinearFn.apply(x, weight, bias)

@@ -1,0 +1,513 @@
+// nf_act8.hip — activations kept in 8 bits between forward and backward, and the weight gradient that reads them.
+//
+// Form: e4m3 codes with one power-of-two scale for every 32 features of a row.  2^k is the smallest power that brings the block's largest finite
+// magnitude to 448 (e4m3's largest) or less, k >= -110; code = x / 2^k rounded to nearest even (the division is exact).  So nothing saturates (but magnitudes above 1.875 2^127), a
+// value is off by at most 2^-4 of itself or 2^-10 2^k, and whatever is not finite becomes NaN, in its own place only.  Codes are rows of
+// Kp = 32 ceil(K / 32) bytes (zeros behind K); scales (k + 127, a byte) lie block by block, [Kp / 32][64 ceil(rows / 64)], so that the reader of
+// a column of blocks finds eight rows' scales in eight adjacent bytes.
+#include "nf_common.h"
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+#define A8_ROWS 64            // rows of a pack tile, of a scale row's padding and of a gradient slab
+
+__device__ __forceinline__ float a8_cv(float v) { return v; }
+struct A8Bf16 { unsigned short u; };
+struct A8F16 { unsigned short u; };
+__device__ __forceinline__ float a8_cv(A8Bf16 v) { return __uint_as_float((unsigned)v.u << 16); }
+__device__ __forceinline__ float a8_cv(A8F16 v) { return (float)__builtin_bit_cast(_Float16, v.u); }
+__device__ __forceinline__ void a8_st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void a8_st(A8Bf16* p, float v) { p->u = __builtin_bit_cast(unsigned short, (__bf16)v); }
+__device__ __forceinline__ void a8_st(A8F16* p, float v) { p->u = __builtin_bit_cast(unsigned short, (_Float16)v); }
+
+// ------------------------------------------------------------------------------------------------
+// pack / unpack: a thread holds 8 adjacent features, four neighbours a block; a workgroup 64 rows x 128 features.
+// ------------------------------------------------------------------------------------------------
+template <typename T, bool VEC> __device__ __forceinline__ void a8_load8(const T* p, int left, float (&v)[8])
+{
+    if (VEC && left >= 8) {
+        alignas(16) T e[8];
+        if (sizeof(T) == 4) { *(uint4*)e = ((const uint4*)p)[0]; *(uint4*)(e + 4) = ((const uint4*)p)[sizeof(T) == 4 ? 1 : 0]; }
+        else *(uint4*)e = *(const uint4*)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = a8_cv(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? a8_cv(p[i]) : 0.f;
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_act8_pack(const T* __restrict__ x, long long xs, int rows, int K, int Kp, int Rp, uint8_t* __restrict__ codes,
+                                                   uint8_t* __restrict__ scales)
+{
+    __shared__ uint8_t sc[4][A8_ROWS];
+    const int c = blockIdx.x * 128 + (threadIdx.x & 15) * 8, r0 = blockIdx.y * A8_ROWS, blk = (threadIdx.x & 15) >> 2;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int lr = it * 16 + (threadIdx.x >> 4), r = r0 + lr;
+        float v[8];
+        const bool in = r < rows && c < K;
+        if (in) a8_load8<T, VEC>(x + (long long)r * xs + c, K - c, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        unsigned top = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned u = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (u < 0x7f800000u) top = max(top, u);
+            else v[i] = __uint_as_float(0x7fc00000u);
+        }
+        top = max(top, (unsigned)__shfl_xor((int)top, 1));
+        top = max(top, (unsigned)__shfl_xor((int)top, 2));
+        // beyond 1.875 2^127 the code's value would be 2^128, which is infinite: such magnitudes are taken as 1.875 2^127 (6 % less at the most)
+        if (top > 0x7f700000u) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((__float_as_uint(v[i]) & 0x7fffffffu) < 0x7f800000u) v[i] = fminf(fmaxf(v[i], -__uint_as_float(0x7f700000u)), __uint_as_float(0x7f700000u));
+        }
+        // top = 1.f 2^e: k = e - 8 while 1.f <= 1.75 (448 = 1.75 2^8), else e - 7
+        const int k = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -110);
+        const float inv = __uint_as_float((unsigned)(127 - k) << 23);
+        if (r < rows && c < Kp) {
+            int lo = 0, hi = 0;
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, lo, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, hi, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
+            *(int2*)(codes + (long long)r * Kp + c) = make_int2(lo, hi);
+        }
+        if ((threadIdx.x & 3) == 0) sc[blk][lr] = (uint8_t)(k + 127);
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const int b = threadIdx.x >> 4, w = threadIdx.x & 15, gb = blockIdx.x * 4 + b;
+        if (gb < Kp / 32) *(unsigned*)(scales + (long long)gb * Rp + r0 + 4 * w) = *(const unsigned*)&sc[b][4 * w];
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K, int Kp, int Rp,
+                                                     T* __restrict__ out, long long os)
+{
+    const int c = blockIdx.x * 128 + (threadIdx.x & 15) * 8, r0 = blockIdx.y * A8_ROWS;
+    if (c >= K) return;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int r = r0 + it * 16 + (threadIdx.x >> 4);
+        if (r >= rows) break;
+        const int2 w = *(const int2*)(codes + (long long)r * Kp + c);
+        const float s = __uint_as_float((unsigned)scales[(long long)(c >> 5) * Rp + r] << 23);
+        float v[8];
+        f32x2 p;
+        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false); v[0] = p.x * s; v[1] = p.y * s;
+        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true); v[2] = p.x * s; v[3] = p.y * s;
+        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false); v[4] = p.x * s; v[5] = p.y * s;
+        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true); v[6] = p.x * s; v[7] = p.y * s;
+        T* o = out + (long long)r * os + c;
+        alignas(16) T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a8_st(&e[i], v[i]);
+        if (VEC && K - c >= 8) {
+            ((uint4*)o)[0] = *(const uint4*)e;
+            if (sizeof(T) == 4) ((uint4*)o)[1] = *(const uint4*)(e + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < K) o[i] = e[i];
+        }
+    }
+}
+
+static size_t a8_kp(int K) { return ((size_t)K + 31) / 32 * 32; }
+static size_t a8_rp(int rows) { return ((size_t)rows + A8_ROWS - 1) / A8_ROWS * A8_ROWS; }
+
+extern "C" size_t nf_act8_code_bytes(int rows, int K) { return rows > 0 && K > 0 ? (size_t)rows * a8_kp(K) : 0; }
+extern "C" size_t nf_act8_scale_bytes(int rows, int K) { return rows > 0 && K > 0 ? a8_rp(rows) * (a8_kp(K) / 32) : 0; }
+
+#define A8_MAX (1 << 30)
+#define A8_GRID(rows, K) dim3((unsigned)((a8_kp(K) + 127) / 128), (unsigned)(a8_rp(rows) / A8_ROWS))
+
+extern "C" int nf_act8_pack(int dtype, const void* x, int64_t x_stride, int rows, int K, uint8_t* codes, uint8_t* scales, nf_stream_t stream)
+{
+    NF_CHECK_ARG(dtype >= 0 && dtype <= 2, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    NF_CHECK_ARG(rows >= 0 && K >= 0 && rows <= A8_MAX && K <= A8_MAX, "bad sizes");
+    if (rows == 0 || K == 0) return NF_OK;
+    NF_CHECK_ARG(x && codes && scales, "null pointer");
+    NF_CHECK_ARG((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "codes and scales must be 16-byte aligned");
+    const int es = dtype == 0 ? 4 : 2;
+    const bool vec = (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0;
+    // a launch's grid has at most 65 535 tiles of rows: longer tensors go in pieces
+    const int step = 65535 * A8_ROWS;
+    for (int r0 = 0; r0 < rows; r0 += step) {
+        const int n = rows - r0 < step ? rows - r0 : step;
+        const dim3 grid = A8_GRID(n, K);
+        const int Kp = (int)a8_kp(K), Rp = (int)a8_rp(rows);
+#define A8_PACK(T)                                                                                                                       \
+    do {                                                                                                                                 \
+        const T* p = (const T*)x + (int64_t)r0 * x_stride;                                                                               \
+        if (vec) hipLaunchKernelGGL((k_act8_pack<T, true>), grid, dim3(256), 0, (hipStream_t)stream, p, (long long)x_stride, n, K, Kp, Rp, \
+                                    codes + (size_t)r0 * Kp, scales + r0);                                                               \
+        else hipLaunchKernelGGL((k_act8_pack<T, false>), grid, dim3(256), 0, (hipStream_t)stream, p, (long long)x_stride, n, K, Kp, Rp,    \
+                                codes + (size_t)r0 * Kp, scales + r0);                                                                   \
+    } while (0)
+        if (dtype == 0) A8_PACK(float);
+        else if (dtype == 1) A8_PACK(A8Bf16);
+        else A8_PACK(A8F16);
+#undef A8_PACK
+        NF_CHECK_LAUNCH();
+    }
+    return NF_OK;
+}
+
+extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* scales, int rows, int K, void* out, int64_t out_stride, nf_stream_t stream)
+{
+    NF_CHECK_ARG(dtype >= 0 && dtype <= 2, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    NF_CHECK_ARG(rows >= 0 && K >= 0 && rows <= A8_MAX && K <= A8_MAX && out_stride >= 0, "bad sizes");
+    if (rows == 0 || K == 0) return NF_OK;
+    NF_CHECK_ARG(out && codes && scales, "null pointer");
+    NF_CHECK_ARG((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "codes and scales must be 16-byte aligned");
+    const int es = dtype == 0 ? 4 : 2;
+    const bool vec = (uintptr_t)out % 16 == 0 && out_stride * es % 16 == 0;
+    const int step = 65535 * A8_ROWS;
+    for (int r0 = 0; r0 < rows; r0 += step) {
+        const int n = rows - r0 < step ? rows - r0 : step;
+        const dim3 grid = A8_GRID(n, K);
+        const int Kp = (int)a8_kp(K), Rp = (int)a8_rp(rows);
+#define A8_UNPACK(T)                                                                                                                         \
+    do {                                                                                                                                     \
+        T* p = (T*)out + (int64_t)r0 * out_stride;                                                                                           \
+        if (vec) hipLaunchKernelGGL((k_act8_unpack<T, true>), grid, dim3(256), 0, (hipStream_t)stream, codes + (size_t)r0 * Kp, scales + r0, n, \
+                                    K, Kp, Rp, p, (long long)out_stride);                                                                    \
+        else hipLaunchKernelGGL((k_act8_unpack<T, false>), grid, dim3(256), 0, (hipStream_t)stream, codes + (size_t)r0 * Kp, scales + r0, n,   \
+                                K, Kp, Rp, p, (long long)out_stride);                                                                        \
+    } while (0)
+        if (dtype == 0) A8_UNPACK(float);
+        else if (dtype == 1) A8_UNPACK(A8Bf16);
+        else A8_UNPACK(A8F16);
+#undef A8_UNPACK
+        NF_CHECK_LAUNCH();
+    }
+    return NF_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// weight gradients from the codes:  dW[m][k] = sum_r dy[r][m] x^[r][k],   db[m] = sum_r dy[r][m]
+//
+// A code with its scale has four significant bits: it is a bf16 number, exactly.  dy is written as a sum of bf16 numbers, exactly too: one for
+// bf16, two for fp16 (11 bits), three for fp32 (24 bits; each the truncation of what is left, so that no rounding can overflow; only what lies below 2^-133, bf16's smallest number, is
+// lost).  So 1 / 2 / 3
+// bf16 matrix instructions with fp32 accumulation give every product exactly, at 16 / 8 / 5.3 times the fp32 matrix rate: the result is that
+// of an fp32 product of dy with the unpacked values, up to the order of the sums.
+//
+// Both operands lie along the outputs, and the reduction runs over the rows: a thread loads 8 rows of 4 (dy) or TK / 32 (codes) adjacent columns, and
+// 8 rows of one column are the 16 bytes that a lane feeds the matrix instruction: the transposition happens in the packing.  A lane's
+// columns go to LDS places 32 apart (column c of quad q at 32 c + q), so that both the writes and the reads run through whole bank rows; which
+// column a matrix row stands for is then settled where the result is stored.
+//
+// Tile: 128 outputs of dy x TK features a workgroup, each of 4 waves a quarter; 64 rows a slab.  The rows are split into slices,
+// whose partial tiles a second launch adds in a fixed order.
+// ------------------------------------------------------------------------------------------------
+#define A8_TM 128
+#define A8_MAX_JOBS 16
+
+struct A8Job { long long out; int dy_col, M, x_col, K, ldo, db, tile0, tiles_k; };     // db: offset of the column sums in the bias blob, -1: none
+struct A8Jobs { int n, ntiles; A8Job j[A8_MAX_JOBS]; };
+
+struct A8Args {
+    const void* dy; long long dys; const uint8_t* codes; const uint8_t* scales;
+    int rows, Kp, Rp, rows_per_slice, nslices;
+    float* out; float* bias;               // slice s at out + s * out_total, bias + s * bias_total
+    long long out_total, bias_total;
+};
+
+template <typename T> struct A8Planes { static constexpr int n = 3; };
+template <> struct A8Planes<A8F16> { static constexpr int n = 2; };
+template <> struct A8Planes<A8Bf16> { static constexpr int n = 1; };
+
+// v = h + (what is returned), h = v with its low 16 bits cleared.  An infinite or NaN v leaves nothing or NaN.
+__device__ __forceinline__ float a8_rest(float v)
+{
+    const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    return h == v ? 0.f : v - h;
+}
+// the upper halves of two words: (low: a, high: b)
+__device__ __forceinline__ unsigned a8_hi2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+
+template <typename T, int TK, bool VEC>
+__global__ void __launch_bounds__(256, 2) k_act8_wgrad(A8Args a, A8Jobs J)
+{
+    constexpr int NP = A8Planes<T>::n, CK = TK / 32;        // CK: adjacent features a thread stages
+    __shared__ uint4 sA[NP][8][A8_TM];
+    __shared__ uint4 sB[8][TK];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wk = wave >> 1;
+    const int slice = blockIdx.x / J.ntiles, tile = blockIdx.x - slice * J.ntiles;
+    int ji = 0;
+    while (ji + 1 < J.n && tile >= J.j[ji + 1].tile0) ++ji;
+    const A8Job job = J.j[ji];
+    const int tm = (tile - job.tile0) / job.tiles_k, tk = (tile - job.tile0) - tm * job.tiles_k;
+    const int m0 = tm * A8_TM, k0 = tk * TK;
+    const int rb = slice * a.rows_per_slice, re = min(a.rows, rb + a.rows_per_slice);
+    const int q = tid & 31, oct = tid >> 5;
+    // columns of this thread; beyond the job's they are read from inside it (the results are not stored)
+    const int cm = m0 + 4 * q, ck = k0 + CK * q;
+    const int ckl = min(ck, (job.K + 31) / 32 * 32 - CK);
+    const T* dyp = (const T*)a.dy + job.dy_col;
+    const uint8_t* xp = a.codes + job.x_col + ckl;
+    const uint8_t* sp = a.scales + (long long)((job.x_col + ckl) >> 5) * a.Rp;
+    f32x16 acc[2][CK / 2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < CK / 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    float bsum[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool with_bias = job.db >= 0 && tk == 0, vec = VEC && job.dy_col % 4 == 0;
+
+    alignas(16) T dv[8][4];
+    unsigned xv[8][CK / 4];
+    uint2 sv;
+    auto fetch = [&](int r0) {
+        const int r = r0 + 8 * oct;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const long long rr = min(r + i, re - 1);
+            const T* p = dyp + rr * a.dys;
+            if (vec && cm + 4 <= job.M) {
+                if (sizeof(T) == 4) *(uint4*)dv[i] = *(const uint4*)(p + cm);
+                else *(uint2*)dv[i] = *(const uint2*)(p + cm);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) dv[i][c] = p[min(cm + c, job.M - 1)];
+            }
+            if (CK == 8) { const uint2 v = *(const uint2*)(xp + rr * a.Kp); xv[i][0] = v.x; xv[i][CK / 4 - 1] = v.y; }
+            else xv[i][0] = *(const unsigned*)(xp + rr * a.Kp);
+        }
+        sv = *(const uint2*)(sp + r);            // (rows are padded to whole slabs)
+    };
+    if (rb < re) fetch(rb);
+    for (int r0 = rb; r0 < re; r0 += A8_ROWS) {
+        const int left = re - (r0 + 8 * oct);    // rows of this thread's eight that exist
+        // dy: planes of the eight rows of each column
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = a8_cv(dv[i][c]);
+            if (left < 8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.f;
+            if (with_bias) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                sA[p][oct][32 * c + q] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
+                if (p + 1 < NP)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
+            }
+        }
+        // codes: two adjacent features a conversion, then rows paired
+        {
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? sv.x >> (8 * i) : sv.y >> (8 * i - 32)) & 0xffu) << 23);
+            if (left < 8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int w = 0; w < CK / 4; ++w) xv[i][w] = i < left ? xv[i][w] : 0u;
+#pragma unroll
+            for (int w = 0; w < CK / 4; ++w) {
+                unsigned lo[8], hi[8];           // features (0, 1) and (2, 3) of the word as bf16 pairs
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    lo[i] = __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i][w], s[i], false));
+                    hi[i] = __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i][w], s[i], true));
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const unsigned* e = c < 2 ? lo : hi;
+                    const unsigned sel = (c & 1) ? 0x07060302u : 0x05040100u;
+                    sB[oct][32 * (4 * w + c) + q] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
+                                                               __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
+                }
+            }
+        }
+        if (r0 + A8_ROWS < re) fetch(r0 + A8_ROWS);      // on its way behind the products
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int o = 2 * ks + (lane >> 5), l = lane & 31;
+            bf16x8 fb[CK / 2];
+#pragma unroll
+            for (int j = 0; j < CK / 2; ++j) fb[j] = __builtin_bit_cast(bf16x8, sB[o][32 * (wk * (CK / 2) + j) + l]);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p)            // the small parts first
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8 fa = __builtin_bit_cast(bf16x8, sA[p][o][32 * (2 * wm + i) + l]);
+#pragma unroll
+                    for (int j = 0; j < CK / 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+    // matrix row i of block b is output 4 i + b of the tile, matrix column j of block b feature CK j + b
+    float* out = a.out + slice * a.out_total + job.out;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int m = m0 + 4 * ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + 2 * wm + i;
+            const int k = k0 + CK * (lane & 31) + wk * (CK / 2);
+            if (m < job.M) {
+                float* o = out + (long long)m * job.ldo + k;
+#pragma unroll
+                for (int j = 0; j < CK / 2; ++j)
+                    if (k + j < job.K) o[j] = acc[i][j][r];
+            }
+        }
+    if (with_bias) {
+        float* sb = (float*)&sB[0][0];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sb[oct * A8_TM + 4 * q + c] = bsum[c];
+        __syncthreads();
+        if (tid < A8_TM && m0 + tid < job.M) {
+            float s = 0.f;
+#pragma unroll
+            for (int o = 0; o < 8; ++o) s += sb[o * A8_TM + tid];
+            a.bias[slice * a.bias_total + job.db + m0 + tid] = s;
+        }
+    }
+}
+
+// Slices added in a fixed order: a thread a quarter of them, then the four quarters.
+__global__ void __launch_bounds__(256) k_act8_fold(const float* __restrict__ part, long long n, int nslices, float* __restrict__ out)
+{
+    __shared__ float s4[4][64];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const long long i = (long long)blockIdx.x * 64 + c;
+    const int per = (nslices + 3) / 4, s0 = g * per, s1 = min(nslices, s0 + per);
+    float v = 0.f;
+    if (i < n) {
+#pragma unroll 8
+        for (int s = s0; s < s1; ++s) v += part[s * n + i];
+    }
+    s4[g][c] = v;
+    __syncthreads();
+    if (g == 0 && i < n) out[i] = (s4[0][c] + s4[1][c]) + (s4[2][c] + s4[3][c]);
+}
+
+static int a8_plan(int njobs, const nf_act8_job_t* jobs, int TK, A8Jobs* J, long long* out_total, long long* bias_total)
+{
+    int tiles = 0;
+    long long out = 0, bias = 0;
+    for (int i = 0; i < njobs; ++i) {
+        const nf_act8_job_t& s = jobs[i];
+        A8Job& j = J->j[i];
+        j.dy_col = s.dy_col; j.M = s.M; j.x_col = s.x_col; j.K = s.K; j.ldo = s.K; j.out = out;
+        j.db = s.bias ? (int)bias : -1;
+        j.tile0 = tiles; j.tiles_k = (s.K + TK - 1) / TK;
+        tiles += ((s.M + A8_TM - 1) / A8_TM) * j.tiles_k;
+        out += (long long)s.M * s.K;
+        if (s.bias) bias += s.M;
+    }
+    J->n = njobs; J->ntiles = tiles;
+    *out_total = out; *bias_total = bias;
+    return tiles;
+}
+
+// The tile's width: 256 features halve the reads of dy; 128 where no job has more.
+static int a8_tk(int njobs, const nf_act8_job_t* jobs)
+{
+    for (int i = 0; i < njobs; ++i)
+        if (jobs[i].K > 128) return 256;
+    return 128;
+}
+
+static int a8_slices(int rows, int tiles)
+{
+    const int slabs = (rows + A8_ROWS - 1) / A8_ROWS;
+    int s = 512 / (tiles > 0 ? tiles : 1);
+    if (s > slabs / 4) s = slabs / 4;
+    if (s < 1) s = 1;
+    const int per = (slabs + s - 1) / s;
+    return per > 0 ? (slabs + per - 1) / per : 1;
+}
+
+static int a8_jobs_ok(const char* who, int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs)
+{
+    const char* bad = nullptr;
+    if (njobs < 1 || njobs > A8_MAX_JOBS || !jobs) bad = "1 to 16 jobs";
+    else if (rows < 0 || rows > A8_MAX || dy_cols < 1 || x_cols < 1) bad = "bad sizes";
+    else
+        for (int i = 0; i < njobs; ++i) {
+            const nf_act8_job_t& j = jobs[i];
+            if (j.M < 1 || j.K < 1 || j.dy_col < 0 || j.x_col < 0 || j.dy_col > dy_cols - j.M || j.x_col > x_cols - j.K) bad = "a job leaves its operands";
+            else if (j.x_col % 32) bad = "a job's first feature must begin a block of 32";
+        }
+    if (bad) { nf_set_error("%s: %s", who, bad); return NF_EINVAL; }
+    return NF_OK;
+}
+
+extern "C" size_t nf_act8_wgrad_workspace_floats(int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs)
+{
+    if (a8_jobs_ok(__func__, rows, dy_cols, x_cols, njobs, jobs)) return 0;
+    A8Jobs J;
+    long long o, b;
+    const int tiles = a8_plan(njobs, jobs, a8_tk(njobs, jobs), &J, &o, &b);
+    const int ns = a8_slices(rows, tiles);
+    return ns > 1 ? (size_t)ns * (size_t)(o + b) : 0;
+}
+
+extern "C" int nf_act8_wgrad(int dtype, const void* dy, int64_t dy_stride, int dy_cols, const uint8_t* codes, const uint8_t* scales, int x_cols, int rows,
+                             int njobs, const nf_act8_job_t* jobs, float* workspace, float* dweights, float* dbias, nf_stream_t stream)
+{
+    NF_CHECK_ARG(dtype >= 0 && dtype <= 2, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    const int rc = a8_jobs_ok(__func__, rows, dy_cols, x_cols, njobs, jobs);
+    if (rc) return rc;
+    A8Jobs J;
+    A8Args a = {};
+    const int TK = a8_tk(njobs, jobs);
+    const int tiles = a8_plan(njobs, jobs, TK, &J, &a.out_total, &a.bias_total);
+    NF_CHECK_ARG(dweights && (a.bias_total == 0 || dbias) && (rows == 0 || (dy && codes && scales)), "null pointer");
+    const int ns = a8_slices(rows, tiles);
+    NF_CHECK_ARG(ns == 1 || workspace, "null workspace (nf_act8_wgrad_workspace_floats)");
+    NF_CHECK_ARG((long long)ns * tiles <= 0x7fffffffLL, "too many tiles");
+    const int slabs = (rows + A8_ROWS - 1) / A8_ROWS;
+    a.dy = dy; a.dys = dy_stride; a.codes = codes; a.scales = scales;
+    a.rows = rows; a.Kp = (int)a8_kp(x_cols); a.Rp = (int)a8_rp(rows); a.nslices = ns;
+    a.rows_per_slice = (slabs + ns - 1) / ns * A8_ROWS;
+    a.out = ns > 1 ? workspace : dweights;
+    a.bias = ns > 1 ? workspace + (size_t)ns * a.out_total : dbias;
+    const int es = dtype == 0 ? 4 : 2;
+    const bool vec = (uintptr_t)dy % (4 * es) == 0 && dy_stride % 4 == 0;
+    const dim3 grid((unsigned)(ns * tiles));
+    hipStream_t st = (hipStream_t)stream;
+#define A8_GO(T, K_)                                                                                       \
+    do {                                                                                                   \
+        if (vec) hipLaunchKernelGGL((k_act8_wgrad<T, K_, true>), grid, dim3(256), 0, st, a, J);             \
+        else hipLaunchKernelGGL((k_act8_wgrad<T, K_, false>), grid, dim3(256), 0, st, a, J);                \
+    } while (0)
+#define A8_GO_K(T) do { if (TK == 256) A8_GO(T, 256); else A8_GO(T, 128); } while (0)
+    if (dtype == 0) A8_GO_K(float);
+    else if (dtype == 1) A8_GO_K(A8Bf16);
+    else A8_GO_K(A8F16);
+#undef A8_GO_K
+#undef A8_GO
+    NF_CHECK_LAUNCH();
+    if (ns > 1) {
+        hipLaunchKernelGGL(k_act8_fold, dim3((unsigned)((a.out_total + 63) / 64)), dim3(256), 0, st, (const float*)a.out, a.out_total, ns, dweights);
+        NF_CHECK_LAUNCH();
+        if (a.bias_total) {
+            hipLaunchKernelGGL(k_act8_fold, dim3((unsigned)((a.bias_total + 63) / 64)), dim3(256), 0, st, (const float*)a.bias, a.bias_total, ns, dbias);
+            NF_CHECK_LAUNCH();
+        }
+    }
+    return NF_OK;
+}

@@ -93,6 +93,9 @@ class _NerfFn(torch.autograd.Function):
         row_sample = torch.arange(n, dtype=torch.int32, device=dev)
         out = torch.zeros(max(n, 1), 4, dtype=torch.float32, device=dev)[:n]
         acts = torch.empty(max(n, 1) * 2432, dtype=torch.float32, device=dev) if need else None
+        ctx.act8 = None
+        if need and net.act_checkpoint is not None:
+            return _NerfFn._forward_act8(ctx, net, xf, sigma_only, packed, X, n_rows, row_sample, out, acts)
         if n > 0:
             check(lib.nf_nerf_mlp_fwd(ptr(packed), cx, cd, ptr(X), ptr(n_rows), n, ptr(row_sample), ptr(out), ptr(acts),
                                       _lib.stream()), "nf_nerf_mlp_fwd")
@@ -106,6 +109,44 @@ class _NerfFn(torch.autograd.Function):
             ctx.save_for_backward(packed, packed_t, X, n_rows, row_sample, out, acts,
                                   layers[0].weight.detach().clone(), layers[4].weight.detach().clone(), layers[9].weight.detach().clone())
         return out[:, 3:4].clone() if sigma_only else out
+
+    @staticmethod
+    def _forward_act8(ctx, net, xf, sigma_only, packed, X, n_rows, row_sample, out, acts):
+        """The training forward with what the backward keeps in 8 bits: the activations (2 432 a row) and the feature row as act8, the ReLU masks
+        as bits.  `acts` and X go back to the allocator when this returns."""
+        from . import act8
+        from .autograd_bwd import _pack_bwd
+        lib = _lib.load()
+        cx, cd, n, dev = net.in_channels_xyz, net.in_channels_dir, xf.shape[0], xf.device
+        layers = net.linear_layers()
+        amask = torch.empty(max(lib.nf_nerf_amask_words(n), 1), dtype=torch.int32, device=dev)
+        if n > 0:
+            packed_n = ops.pack_nerf_n(packed, cx, cd)
+            check(lib.nf_nerf_mlp_fwd_n2(ptr(packed_n), cx, cd, ptr(X), ptr(n_rows), n, ptr(row_sample), ptr(out), ptr(acts), ptr(amask), _lib.stream()),
+                  "nf_nerf_mlp_fwd_n2")
+        ctx.act8 = (act8.pack(acts[:n * 2432].view(n, 2432)), act8.pack(xf[:, :cx]), act8.pack(xf[:, cx:]))
+        ctx.net, ctx.sigma_only, ctx.n, ctx.x_needs_grad = net, sigma_only, n, bool(ctx.needs_input_grad[1])
+        ctx.save_for_backward(packed, _pack_bwd(net, cx, cd, dev), amask, n_rows, row_sample, out, None,
+                              layers[0].weight.detach().clone(), layers[4].weight.detach().clone(), layers[9].weight.detach().clone())
+        return out[:, 3:4].clone() if sigma_only else out
+
+    @staticmethod
+    def _wgrad_act8(ctx, dpre):
+        """The 12 weight and 12 bias gradients from the packed activations (first column of dpre, outputs, first feature, features, bias)."""
+        from . import act8
+        cx, cd = ctx.net.in_channels_xyz, ctx.net.in_channels_dir
+        acts8, xyz8, dir8 = ctx.act8
+        hidden = [1, 2, 3, 4, 5, 6, 7]
+        jobs = [(256 * l, 256, 256 * (l - 1), 256, True) for l in hidden]
+        jobs += [(8 * 256, 256, 7 * 256, 256, True), (9 * 256, 128, 8 * 256, 256, True), (2435, 1, 7 * 256, 256, True), (2432, 3, 9 * 256, 128, True)]
+        r = act8.wgrad_jobs(dpre, acts8, jobs)
+        first, skip = act8.wgrad_jobs(dpre, xyz8, [(0, 256, 0, cx, True), (4 * 256, 256, 0, cx, False)])
+        view, = act8.wgrad_jobs(dpre, dir8, [(9 * 256, 128, 0, cd, False)])
+        gw = [first[0]] + [q[0] for q in r[:7]] + [q[0] for q in r[7:]]
+        gw[4] = torch.cat([skip[0], gw[4]], 1)
+        gw[9] = torch.cat([gw[9], view[0]], 1)
+        gb = [first[1]] + [q[1] for q in r]
+        return gw, gb
 
     @staticmethod
     def backward(ctx, g):
@@ -130,20 +171,14 @@ class _NerfFn(torch.autograd.Function):
         else:
             d_rs.copy_(g.detach().float())
         dpre = torch.empty(n, DPRE, dtype=torch.float32, device=dev)
-        check(lib.nf_nerf_mlp_bwd_n(ptr(packed), ptr(packed_t), cx, cd, ptr(acts), ptr(n_rows), n, ptr(row_sample), ptr(out),
-                                  ptr(d_rs), ptr(dpre), st), "nf_nerf_mlp_bwd_n")
-        nsl = 22          # 46 tiles x 22 row slices = 1 012 waves: one 128 x 128 tile per wave, one wave per SIMD
-        blob = torch.empty(lib.nf_nerf_wgrad_floats(cx, cd), dtype=torch.float32, device=dev)
-        wsp = torch.empty(lib.nf_nerf_wgrad_workspace_floats(cx, cd, nsl), dtype=torch.float32, device=dev)
-        colsum = torch.empty(DPRE, dtype=torch.float32, device=dev)
-        check(lib.nf_nerf_wgrad(ptr(dpre), ptr(acts), ptr(X), cx, cd, n, nsl, ptr(wsp), ptr(blob), ptr(colsum), st), "nf_nerf_wgrad")
-        gw, o = [], 0
-        for l in layers:
-            k = l.weight.numel()
-            gw.append(blob[o:o + k].view_as(l.weight))
-            o += k
-        gb = [colsum[k * 256:(k + 1) * 256] for k in range(8)]
-        gb += [colsum[8 * 256:9 * 256], colsum[9 * 256:9 * 256 + 128], colsum[2435:2436], colsum[2432:2435]]
+        if ctx.act8 is not None:         # X holds the mask words here
+            check(lib.nf_nerf_mlp_bwd_n2(ptr(packed), ptr(packed_t), cx, cd, ptr(X), ptr(n_rows), n, ptr(row_sample), ptr(out), ptr(d_rs),
+                                         ptr(dpre), st), "nf_nerf_mlp_bwd_n2")
+            gw, gb = _NerfFn._wgrad_act8(ctx, dpre)
+        else:
+            check(lib.nf_nerf_mlp_bwd_n(ptr(packed), ptr(packed_t), cx, cd, ptr(acts), ptr(n_rows), n, ptr(row_sample), ptr(out),
+                                        ptr(d_rs), ptr(dpre), st), "nf_nerf_mlp_bwd_n")
+            gw, gb = _NerfFn._wgrad(lib, st, layers, dpre, acts, X, cx, cd, n)
         dx = None
         for i in unused:
             gw[i] = gb[i] = None
@@ -156,13 +191,40 @@ class _NerfFn(torch.autograd.Function):
                 dx = dx[:, :cx].contiguous()
         return (None, dx, None) + tuple(gw) + tuple(gb)
 
+    @staticmethod
+    def _wgrad(lib, st, layers, dpre, acts, X, cx, cd, n):
+        from .autograd_bwd import DPRE
+        dev = dpre.device
+        nsl = 22          # 46 tiles x 22 row slices = 1 012 waves: one 128 x 128 tile per wave, one wave per SIMD
+        blob = torch.empty(lib.nf_nerf_wgrad_floats(cx, cd), dtype=torch.float32, device=dev)
+        wsp = torch.empty(lib.nf_nerf_wgrad_workspace_floats(cx, cd, nsl), dtype=torch.float32, device=dev)
+        colsum = torch.empty(DPRE, dtype=torch.float32, device=dev)
+        check(lib.nf_nerf_wgrad(ptr(dpre), ptr(acts), ptr(X), cx, cd, n, nsl, ptr(wsp), ptr(blob), ptr(colsum), st), "nf_nerf_wgrad")
+        gw, o = [], 0
+        for l in layers:
+            k = l.weight.numel()
+            gw.append(blob[o:o + k].view_as(l.weight))
+            o += k
+        gb = [colsum[k * 256:(k + 1) * 256] for k in range(8)]
+        gb += [colsum[8 * 256:9 * 256], colsum[9 * 256:9 * 256 + 128], colsum[2435:2436], colsum[2432:2435]]
+        return gw, gb
+
 
 class NeRF(nn.Module):
     """models/nerf.py:42-124 (D = 8, W = 256, skips = [4]): parameters with the reference's layer names; forward on the
-    fp32-MFMA kernels."""
+    fp32-MFMA kernels.
 
-    def __init__(self, D=8, W=256, in_channels_xyz=63, in_channels_dir=27, skips=(4,)):
+    act_checkpoint="e4m3" (not in the reference): what a training forward keeps for the weight gradients — the activations and the feature row — is
+    kept in 8 bits (act8): 3.1 KB a row (masks included) instead of 10.8 KB.  Outputs and dL/dx are the fp32 path's (heads summed in another
+    order: equal to the last bits); the weight gradients are those of the rounded activations.  For the default feature row (198 + 54 features)."""
+
+    def __init__(self, D=8, W=256, in_channels_xyz=63, in_channels_dir=27, skips=(4,), act_checkpoint=None):
         super().__init__()
+        if act_checkpoint not in (None, "e4m3"):
+            raise ValueError(f"act_checkpoint must be None or 'e4m3', not {act_checkpoint!r}")
+        if act_checkpoint is not None and ((in_channels_xyz + 7) // 8, (in_channels_dir + 7) // 8) != (25, 7):
+            raise NotImplementedError("act_checkpoint: the forward that leaves the ReLU masks as bits serves the default feature row (198 + 54)")
+        self.act_checkpoint = act_checkpoint
         if D != 8 or W != 256 or tuple(skips) != (4,):
             raise NotImplementedError("the MFMA kernel implements the reference's D=8, W=256, skips=[4] network")
         self.D, self.W, self.skips = D, W, list(skips)

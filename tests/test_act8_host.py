@@ -1,0 +1,73 @@
+"""Refusals of the 8-bit activation checkpoints, on the host."""
+import ctypes
+
+import pytest
+import torch
+
+from neurofluid_amd import act8
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def fake(rows, K):
+    return act8.Act8(t(rows * ((K + 31) // 32 * 32), dtype=torch.uint8), t(64, dtype=torch.uint8), (rows, K), torch.float32)
+
+
+@pytest.mark.parametrize("x, err", [(t(4, 5, dtype=torch.float64), TypeError), (t(4, 5, dtype=torch.int32), TypeError), (torch.tensor(1.0), ValueError),
+                                    (t(4, 5), RuntimeError), (t(1, 1).expand((1 << 30) + 1, 1), ValueError)])
+def test_pack_refuses(x, err):
+    with pytest.raises(err):
+        act8.pack(x)
+
+
+@pytest.mark.parametrize("dy, ck, err", [
+    (t(4, 5, dtype=torch.float64), fake(4, 6), TypeError), (t(4, 5), t(4, 6), TypeError), (t(3, 5), fake(4, 6), ValueError),
+    (t(4, 0), fake(4, 6), ValueError), (t(4, 5), fake(4, 0), ValueError), (t(4, 5), fake(4, 6), RuntimeError)])
+def test_wgrad_refuses(dy, ck, err):
+    with pytest.raises(err):
+        act8.wgrad(dy, ck)
+
+
+def test_unpack_refuses():
+    with pytest.raises(TypeError):
+        fake(2, 3).unpack(torch.float64)
+
+
+@pytest.mark.parametrize("x, w, b, err", [
+    (t(4, 5, dtype=torch.bfloat16), t(3, 5), None, TypeError), (t(4, 5), t(3, 5, dtype=torch.float16), None, TypeError),
+    (t(4, 5), t(3, 6), None, ValueError), (t(4, 5), t(5), None, ValueError), (t(4, 5), t(3, 5), t(4), ValueError), (t(4, 5), t(3, 5), t(3, 1), ValueError),
+    (t(4, 5), t(0, 5), None, ValueError), (t(4, 5), t(3, 5), t(3), RuntimeError)])
+def test_linear_refuses(x, w, b, err):
+    with pytest.raises(err):
+        act8.linear(x, w, b)
+
+
+def test_nerf_refuses():
+    from neurofluid_amd.nerf import NeRF
+    with pytest.raises(ValueError):
+        NeRF(in_channels_xyz=198, in_channels_dir=54, act_checkpoint="int4")
+    with pytest.raises(NotImplementedError):
+        NeRF(in_channels_xyz=63, in_channels_dir=27, act_checkpoint="e4m3")
+    a, b = NeRF(in_channels_xyz=198, in_channels_dir=54, act_checkpoint="e4m3"), NeRF(in_channels_xyz=198, in_channels_dir=54)
+    assert list(a.state_dict()) == list(b.state_dict())
+
+
+def test_c_entries_refuse():
+    from neurofluid_amd import _lib, build
+    build.build()
+    lib = _lib.load()
+    assert lib.nf_act8_code_bytes(3, 33) == 3 * 64 and lib.nf_act8_scale_bytes(65, 33) == 128 * 2 and lib.nf_act8_code_bytes(0, 4) == 0
+    assert lib.nf_act8_pack(5, None, 0, 1, 1, None, None, None) < 0 and b"dtype" in lib.nf_last_error()
+    assert lib.nf_act8_pack(0, None, 4, 4, 4, None, None, None) < 0 and b"null" in lib.nf_last_error()
+    assert lib.nf_act8_pack(0, None, 4, -1, 4, None, None, None) < 0
+    assert lib.nf_act8_unpack(0, None, None, 4, 4, None, 4, None) < 0
+    job = lambda *a: (_lib.Act8Job * 1)(_lib.Act8Job(*a))
+    for bad in (job(0, 5, 0, 4, 1), job(1, 4, 0, 4, 1), job(0, 4, 16, 4, 1), job(0, 4, 0, 65, 1), job(-1, 2, 0, 4, 1), job(0, 0, 0, 4, 1), job(2 ** 31 - 1, 2, 0, 4, 1)):
+        assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 1, bad, None, None, None, None) < 0
+        assert lib.nf_act8_wgrad_workspace_floats(8, 4, 64, 1, bad) == 0
+    ok = job(0, 4, 32, 4, 1)
+    assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 0, ok, None, None, None, None) < 0
+    assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 1, ok, None, None, None, None) < 0 and b"null" in lib.nf_last_error()
+    assert lib.nf_act8_wgrad_workspace_floats(100000, 4, 64, 1, ok) > 0
