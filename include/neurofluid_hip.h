@@ -591,8 +591,8 @@ int nf_trans_step(const nf_trans_step_t* s /*[host]*/, const float* pos, const f
  * The stretch products carry states over long distances: gates are meant to be decays (|A| <= 1), larger ones overflow there sooner than
  * step by step.  Results repeat bit for bit.
  * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, nw; *state_floats = the size
- * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_floats =
- * nf_scan_workspace_floats(s, backward) floats.  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
+ * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_bytes =
+ * nf_scan_workspace_bytes(s, backward) bytes, 8-byte aligned, for this call alone.  T <= 2^30, D <= 2^20, step strides < 2^19 elements or so (a tile's rows span less than 2^31 bytes).  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
  * h0, states (and sid).
  * row_splits (device, n_seq + 1, ascending): B = 1 and the T rows hold n_seq sequences behind one another, h0 / h_last / g_last / dh0 have
  * one row for each (an empty sequence passes them through); h, dx, dgate are zero on rows that belong to none.  sid: T ints, filled by the
@@ -607,10 +607,10 @@ typedef struct {
     void* h; float* h_last; float* states /*forward: or NULL*/; int32_t* sid /*packed*/;
     void* dgate /*or NULL*/; void* dx /*or NULL*/; float* dh0 /*or NULL*/;
     int vec, cg, nw;
-    float* workspace; size_t workspace_floats;
+    void* workspace; size_t workspace_bytes;
 } nf_scan_t;
 int nf_scan_plan(nf_scan_t* s /*[host]*/, size_t* state_floats /*[host]*/);
-size_t nf_scan_workspace_floats(const nf_scan_t* s /*[host]*/, int backward);
+size_t nf_scan_workspace_bytes(const nf_scan_t* s /*[host]*/, int backward);
 int nf_scan_fwd(const nf_scan_t* s /*[host]*/, nf_stream_t stream);
 int nf_scan_bwd(const nf_scan_t* s /*[host]*/, nf_stream_t stream);
 /* One step for `rows` independent states: next = A state + x (fp32, row strides in elements; next may be state itself), h = next in

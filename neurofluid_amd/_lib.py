@@ -32,7 +32,7 @@ class Scan(ctypes.Structure):
                [(k, c_void_p) for k in ("row_splits", "gate", "x", "g", "h0", "g_last")] + \
                [(k, c_int64) for k in ("gate_sb", "gate_st", "x_sb", "x_st", "g_sb", "g_st")] + \
                [(k, c_void_p) for k in ("h", "h_last", "states", "sid", "dgate", "dx", "dh0")] + \
-               [(k, c_int) for k in ("vec", "cg", "nw")] + [("workspace", c_void_p), ("workspace_floats", c_size_t)]
+               [(k, c_int) for k in ("vec", "cg", "nw")] + [("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
 class Act8Job(ctypes.Structure):
@@ -178,7 +178,7 @@ PROTOTYPES = {
     "nf_e2e_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, ctypes.POINTER(c_float), ctypes.POINTER(c_float), c_float,
                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nf_scan_plan": (c_int, [ctypes.POINTER(Scan), ctypes.POINTER(c_size_t)]),
-    "nf_scan_workspace_floats": (c_size_t, [ctypes.POINTER(Scan), c_int]),
+    "nf_scan_workspace_bytes": (c_size_t, [ctypes.POINTER(Scan), c_int]),
     "nf_scan_fwd": (c_int, [ctypes.POINTER(Scan), c_void_p]),
     "nf_scan_bwd": (c_int, [ctypes.POINTER(Scan), c_void_p]),
     "nf_scan_step": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,

@@ -1,77 +1,79 @@
 // nf_scan.hip — entry points of the gated linear recurrence (kernels: nf_scan.h).
-//
-// Where the parallelism comes from.  A (sequence, block of channels) is a chain; its tiles follow one another.
-//   many chains: one workgroup (NW = 4 waves on a tile) or one wave (NW = 1, four chains a workgroup) walks a whole chain, each
-//     tensor is read and written once;
-//   few chains: the time axis is cut into chunks of whole tiles.  One launch reduces every chunk to (P, H), a small one carries the states
-//     through the chunks in order, a third runs the chunks from the states that enter them.  The gate and the input are read twice.
 #include "nf_scan.h"
 #include <math.h>
 
-static int scan_tile(int cg, int nw) { return nw * (64 / cg) * NF_SCAN_TPT; }
-
-// Chunks a chain is cut into: enough workgroups for four per CU.
-static int scan_chunks(const nf_scan_t* s)
-{
-    const int tile = scan_tile(s->cg, s->nw), ntiles = (s->T + tile - 1) / tile;
-    const long long units = (long long)s->B * ((s->D + s->cg * s->vec - 1) / (s->cg * s->vec));
-    if (s->nw == 1 || ntiles <= 4 || units >= 512) return 1;
-    const long long want = (1024 + units - 1) / units;
-    const int per = (int)((ntiles + want - 1) / want);
-    return (ntiles + per - 1) / per;
-}
+static int scan_waves(const nf_scan_t* s) { return s->nw < 0 ? -s->nw : s->nw; }
+static int scan_tile(const nf_scan_t* s) { return scan_waves(s) * (64 / s->cg) * NF_SCAN_TPT(s->vec); }
+static long long scan_blocks(const nf_scan_t* s) { return (s->D + s->cg * s->vec - 1) / (s->cg * s->vec); }
 
 static int scan_check(const nf_scan_t* s, const char* who)
 {
     if (!s) { nf_set_error("%s: null descriptor", who); return NF_EINVAL; }
     if (s->dtype < 0 || s->dtype > 2) { nf_set_error("%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)", who); return NF_EINVAL; }
-    if (s->B < 0 || s->T < 0 || s->D < 1) { nf_set_error("%s: bad sizes", who); return NF_EINVAL; }
+    if (s->B < 0 || s->T < 0 || s->D < 1 || s->T > NF_SCAN_MAX_STEPS || s->D > NF_SCAN_MAX_CHANNELS) { nf_set_error("%s: bad sizes", who); return NF_EINVAL; }
     if (s->row_splits && (s->B != 1 || s->n_seq < 0)) { nf_set_error("%s: packed rows come as one batch", who); return NF_EINVAL; }
     return NF_OK;
 }
 
 static bool scan_plan_ok(const nf_scan_t* s)
 {
-    return (s->vec == 1 || s->vec == 2) && (s->cg == 32 || s->cg == 16 || s->cg == 8 || s->cg == 2) && (s->nw == 1 || s->nw == 4) &&
-           (s->vec == 1 || s->D % 2 == 0);
+    const bool lanes = s->vec == 4 ? (s->cg == 16 || s->cg == 8 || s->cg == 4 || s->cg == 1) : ((s->vec == 2 || s->vec == 1) && (s->cg == 32 || s->cg == 8 || s->cg == 2));
+    return lanes && (s->nw == 1 || s->nw == 4 || s->nw == -NF_SCAN_CW) && s->D % s->vec == 0;
 }
 
-// true if every row that (base, strides) reaches can be read two elements at a time
-static bool scan_pairs(const void* p, int64_t sb, int64_t st, int size) { return (uintptr_t)p % (2 * size) == 0 && sb % 2 == 0 && st % 2 == 0; }
+// elements that every row which (base, strides) reaches can be read at a time: 4, 2 or 1
+static int scan_vec(const void* p, int64_t sb, int64_t st, int size)
+{
+    int v = 4;
+    while (v > 1 && ((uintptr_t)p % (v * size) || sb % v || st % v)) v /= 2;
+    return v;
+}
 
+// Lanes: as many channels a block as D has, 64 at the most.  Waves: a chain of few steps, or one of thousands, keeps to a wave (no
+// barrier); below 1 024 chains the tiles of a chain go to workgroups of their own.
 extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
 {
     const int rc = scan_check(s, __func__);
     if (rc) return rc;
     const int es = s->dtype == 0 ? 4 : 2, gs = (s->dtype == 0 || s->gate32) ? 4 : 2;
-    s->vec = (s->D % 2 == 0 && scan_pairs(s->x, s->x_sb, s->x_st, es) && (s->shared || scan_pairs(s->gate, s->gate_sb, s->gate_st, gs))) ? 2 : 1;
-    s->cg = 32;
-    const int cgs[3] = {2, 8, 16};
-    for (int i = 2; i >= 0; --i)
-        if (cgs[i] * s->vec >= s->D) s->cg = cgs[i];
-    const int nblk = (s->D + s->cg * s->vec - 1) / (s->cg * s->vec);
-    const int t1 = scan_tile(s->cg, 1);
-    s->nw = (!s->row_splits && ((long long)s->B * nblk >= 4096 || s->T <= 2 * t1)) ? 1 : 4;
-    const int tile = scan_tile(s->cg, s->nw);
+    int v = scan_vec(s->x, s->x_sb, s->x_st, es);
+    if (!s->shared) { const int vg = scan_vec(s->gate, s->gate_sb, s->gate_st, gs); v = vg < v ? vg : v; }
+    while (s->D % v) v /= 2;
+    s->vec = v;
+    if (v == 4) s->cg = s->D <= 4 ? 1 : s->D <= 16 ? 4 : s->D <= 32 ? 8 : 16;
+    else s->cg = s->D <= 2 * v ? 2 : s->D <= 8 * v ? 8 : 32;
+    const long long chains = (long long)s->B * scan_blocks(s);
+    s->nw = 1;
+    const int t1 = scan_tile(s);
+    if (s->T > t1 && (s->row_splits || (chains < 4096 && s->T > 2 * t1))) {
+        s->nw = 4;
+        if (s->T > scan_tile(s) && chains < 1024) s->nw = -NF_SCAN_CW;
+    }
+    const int tile = scan_tile(s);
     if (state_floats) *state_floats = (size_t)s->B * ((s->T + tile - 1) / tile) * s->D;
     return NF_OK;
 }
 
-// workspace: [agg | carry] when the time axis is cut, then the per-block sums of a shared gate's gradient
-static void scan_workspace(const nf_scan_t* s, int backward, size_t* agg, size_t* carry, size_t* part)
+// workspace, in 8-byte words: [tile | group | set entries | ticket] of the chained kernels, then the per-block sums of a shared gate's gradient
+struct ScanWs { size_t tile, group, set, part; size_t entries() const { return tile + group + set; } size_t words() const { return (entries() ? entries() + 1 : 0) + (part + 1) / 2; } };
+static ScanWs scan_workspace(const nf_scan_t* s, int backward)
 {
-    const int nchunk = scan_chunks(s), nblk = (s->D + s->cg * s->vec - 1) / (s->cg * s->vec);
-    *agg = nchunk > 1 ? (size_t)s->B * nchunk * 2 * s->D : 0;
-    *carry = nchunk > 1 ? (size_t)s->B * nchunk * s->D : 0;
-    *part = (backward && s->shared && s->dgate && nblk > 1) ? (size_t)nblk * s->B * s->T : 0;
+    ScanWs w = {0, 0, 0, 0};
+    if (s->nw < 0) {
+        const int tile = scan_tile(s);
+        const size_t per = (size_t)s->B * scan_blocks(s) * s->cg * s->vec, nt = (s->T + tile - 1) / tile;
+        w.tile = nt * per;
+        w.group = (nt + NF_SCAN_FAN - 1) / NF_SCAN_FAN * per;
+        w.set = (nt + NF_SCAN_FAN * NF_SCAN_FAN - 1) / (NF_SCAN_FAN * NF_SCAN_FAN) * per;
+    }
+    if (backward && s->shared && s->dgate && scan_blocks(s) > 1) w.part = (size_t)scan_blocks(s) * s->B * s->T;
+    return w;
 }
 
-extern "C" size_t nf_scan_workspace_floats(const nf_scan_t* s, int backward)
+extern "C" size_t nf_scan_workspace_bytes(const nf_scan_t* s, int backward)
 {
     if (scan_check(s, __func__) || !scan_plan_ok(s)) return 0;
-    size_t a, c, p;
-    scan_workspace(s, backward, &a, &c, &p);
-    return a + c + p;
+    return 8 * scan_workspace(s, backward).words();
 }
 
 // The sequence of every packed row (-1: before the first or behind the last), by bisection of the splits; the final states of empty
@@ -100,27 +102,10 @@ __global__ void __launch_bounds__(256) k_scan_empty(const int64_t* __restrict__ 
     if (a >= b) dst[e] = src ? src[e] : 0.f;
 }
 
-// The states that enter the chunks, in order.  One thread per channel of a chain; the loads do not depend on the state.
-__global__ void __launch_bounds__(64) k_scan_carry(const float* __restrict__ agg, const float* __restrict__ init, const int* __restrict__ sid, int B,
-                                                   int D, int T, int nchunk, int steps, int reverse, int backward, float* __restrict__ carry)
+// The chain's entries are set to "empty", the counter of tiles to 0 (a kernel: a memset node in a captured graph has given wrong results).
+__global__ void __launch_bounds__(256) k_scan_clear(unsigned long long* __restrict__ w, size_t entries)
 {
-    const int d = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-    if (d >= D) return;
-    float c = init ? init[(long long)b * D + d] : 0.f;
-    auto at = [&](int j) { return (j < 0 || j >= T) ? -2 : sid[reverse ? T - 1 - j : j]; };
-#pragma unroll 8
-    for (int i = 0; i < nchunk; ++i) {
-        const int k = backward ? nchunk - 1 - i : i;
-        const long long o = (long long)b * nchunk + k;
-        const float P = agg[o * 2 * D + d], H = agg[(o * 2 + 1) * D + d];
-        carry[o * D + d] = c;
-        bool closed = false;
-        if (sid) {                       // does a sequence begin (backwards: end) inside the chunk?
-            const int j0 = k * steps, j1 = min(T, j0 + steps) - 1;
-            closed = backward ? at(j1 + 1) != at(j0) : at(j0 - 1) != at(j1);
-        }
-        c = closed ? H : fmaf(P, c, H);
-    }
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i <= entries; i += (size_t)gridDim.x * 256) w[i] = i < entries ? NF_SCAN_EMPTY : 0ull;
 }
 
 __global__ void __launch_bounds__(256) k_scan_fold(const float* __restrict__ part, int nblk, long long n, int type, void* __restrict__ out)
@@ -160,45 +145,46 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     if (!s->gate || !s->x || (backward ? !s->states : !s->h)) { nf_set_error("%s: null pointer", who); return NF_EINVAL; }
     if (packed && !s->sid) { nf_set_error("%s: packed rows need the row buffer (sid)", who); return NF_EINVAL; }
     const int es = s->dtype == 0 ? 4 : 2, gs = (s->dtype == 0 || s->gate32) ? 4 : 2;
-    if (s->vec == 2 && !(scan_pairs(s->x, s->x_sb, s->x_st, es) && (s->shared || scan_pairs(s->gate, s->gate_sb, s->gate_st, gs)) &&
-                         (!backward || !s->g || scan_pairs(s->g, s->g_sb, s->g_st, es)))) {
-        nf_set_error("%s: the plan reads two elements at a time, a tensor is not aligned for it", who);
+    if (scan_vec(s->x, s->x_sb, s->x_st, es) < s->vec || (!s->shared && scan_vec(s->gate, s->gate_sb, s->gate_st, gs) < s->vec) ||
+        (backward && s->g && scan_vec(s->g, s->g_sb, s->g_st, es) < s->vec) || (!backward && (uintptr_t)s->h % (s->vec * es)) ||
+        (backward && ((uintptr_t)s->dx % (s->vec * es) || (!s->shared && (uintptr_t)s->dgate % (s->vec * gs))))) {
+        nf_set_error("%s: the plan reads %d elements at a time, a tensor is not aligned for it", who, s->vec);
         return NF_EINVAL;
     }
     NfScanArgs a = {};
     a.gate = s->gate; a.x = s->x; a.g = s->g; a.h0 = s->h0; a.g_last = s->g_last; a.h = s->h; a.h_last = s->h_last; a.states = s->states;
     a.dgate = s->dgate; a.dx = s->dx; a.dh0 = s->dh0; a.sid = packed ? s->sid : nullptr;
-    a.gate_sb = s->gate_sb; a.gate_st = s->gate_st; a.x_sb = s->x_sb; a.x_st = s->x_st; a.g_sb = s->g_sb; a.g_st = s->g_st;
-    a.B = s->B; a.T = s->T; a.D = s->D;
-    const int tile = scan_tile(s->cg, s->nw);
-    a.nblk = (s->D + s->cg * s->vec - 1) / (s->cg * s->vec);
-    a.ntiles = (s->T + tile - 1) / tile;
-    a.nchunk = scan_chunks(s);
-    a.tiles_per_chunk = (a.ntiles + a.nchunk - 1) / a.nchunk;
-    a.gate32 = s->gate32 != 0; a.shared = s->shared != 0; a.log_gate = s->log_gate != 0; a.reverse = s->reverse != 0;
-    if ((long long)a.B * a.nblk * a.nchunk > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
-    size_t n_agg, n_carry, n_part;
-    scan_workspace(s, backward, &n_agg, &n_carry, &n_part);
-    if (s->workspace_floats < n_agg + n_carry + n_part || (n_agg + n_carry + n_part && !s->workspace)) {
-        nf_set_error("%s: workspace too small (nf_scan_workspace_floats)", who);
+    const int tile = scan_tile(s);
+    const int64_t far = 0x7fffffff / tile / 4;
+    const int64_t gate_st = s->T > 1 ? s->gate_st : 0, x_st = s->T > 1 ? s->x_st : 0, g_st = s->T > 1 ? s->g_st : 0;
+    if (gate_st < 0 || x_st < 0 || g_st < 0 || gate_st > far || x_st > far || g_st > far) {
+        nf_set_error("%s: steps of a tensor lie too far apart (copy it)", who);
         return NF_EINVAL;
     }
-    float* agg = s->workspace;
-    float* carry = agg + n_agg;
-    a.dgate_part = n_part ? carry + n_carry : nullptr;
+    a.gate_sb = s->gate_sb * gs; a.x_sb = s->x_sb * es; a.g_sb = s->g_sb * es;
+    a.gate_st = (int)(gate_st * gs); a.x_st = (int)(x_st * es); a.g_st = (int)(g_st * es);
+    a.B = s->B; a.T = s->T; a.D = s->D;
+    a.nblk = (int)scan_blocks(s);
+    a.ntiles = (s->T + tile - 1) / tile;
+    a.gate32 = s->gate32 != 0; a.shared = s->shared != 0; a.log_gate = s->log_gate != 0; a.reverse = s->reverse != 0;
+    if ((long long)a.B * a.nblk * (s->nw < 0 ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
+    const ScanWs ws = scan_workspace(s, backward);
+    const size_t n_part = ws.part;
+    if (s->workspace_bytes < 8 * ws.words() || (ws.words() && (!s->workspace || (uintptr_t)s->workspace % 8))) {
+        nf_set_error("%s: workspace too small or unaligned (nf_scan_workspace_bytes)", who);
+        return NF_EINVAL;
+    }
+    unsigned long long* words = (unsigned long long*)s->workspace;
+    a.ws_tile = words; a.ws_group = words + ws.tile; a.ws_set = a.ws_group + ws.group; a.ticket = (int*)(words + ws.entries());
+    a.dgate_part = n_part ? (float*)(words + (ws.entries() ? ws.entries() + 1 : 0)) : nullptr;
     if (packed && !backward) {
         hipLaunchKernelGGL(k_scan_rows, dim3((unsigned)((s->T + 255) / 256)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->sid);
         NF_CHECK_LAUNCH();
     }
-    if (a.nchunk > 1) {
-        NfScanArgs r = a;
-        r.only_agg = 1; r.agg = agg;
-        if (!scan_go(s, r, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
+    if (ws.entries()) {
+        const size_t blocks = (ws.entries() + 256) / 256;
+        hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, words, ws.entries());
         NF_CHECK_LAUNCH();
-        hipLaunchKernelGGL(k_scan_carry, dim3((s->D + 63) / 64, s->B), dim3(64), 0, st, (const float*)agg, packed ? (const float*)nullptr : init, a.sid, s->B,
-                           s->D, s->T, a.nchunk, a.tiles_per_chunk * tile, a.reverse, backward, carry);
-        NF_CHECK_LAUNCH();
-        a.carry = carry;
     }
     if (!scan_go(s, a, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
     NF_CHECK_LAUNCH();

@@ -14,12 +14,14 @@ from . import _lib, ops
 from ._lib import check, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_MAX_STEPS = 1 << 30
+_MAX_STEPS, _MAX_CHANNELS, _MAX_STRIDE = 1 << 30, 1 << 20, 1 << 18
 
 
 def _rows(t):
-    """t with adjacent channels (a copy if they are not)."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """t with adjacent channels and steps that are not too far apart (a copy if they are)."""
+    if (t.shape[-1] == 1 or t.stride(-1) == 1) and (t.stride(-2) <= _MAX_STRIDE or t.shape[-2] <= 1):
+        return t
+    return t.contiguous()
 
 
 def _check(gate, x, what):
@@ -54,8 +56,8 @@ def _describe(gate, x, row_splits, log_gate, reverse):
 
 
 def _workspace(lib, s, backward, dev):
-    s.workspace_floats = lib.nf_scan_workspace_floats(ctypes.byref(s), backward)
-    ws = torch.empty(s.workspace_floats, dtype=torch.float32, device=dev) if s.workspace_floats else None
+    s.workspace_bytes = lib.nf_scan_workspace_bytes(ctypes.byref(s), backward)
+    ws = torch.empty(s.workspace_bytes, dtype=torch.uint8, device=dev) if s.workspace_bytes else None
     s.workspace = ptr(ws)
     return ws
 
@@ -114,8 +116,8 @@ class _ScanFn(torch.autograd.Function):
                 y = None
                 if g is not None:
                     y = _rows(g.detach())
-                    if s.vec == 2 and (y.data_ptr() % (2 * y.element_size()) or any(v % 2 for v in y.stride()[:-1])):
-                        y = y.contiguous().clone() if y.is_contiguous() else y.contiguous()
+                    if y.data_ptr() % (s.vec * y.element_size()) or any(v % s.vec for v in y.stride()[:-1]):
+                        y = y.clone(memory_format=torch.contiguous_format)
                     s.g_sb, s.g_st = (0, y.stride(0)) if row_splits is not None else (y.stride(0), y.stride(1))
                 s.g, s.h0, s.g_last, s.states, s.sid = ptr(y), ptr(h0_), ptr(gl), ptr(states), ptr(sid)
                 s.dgate, s.dx, s.dh0 = ptr(dgate), ptr(dx), ptr(dh0)
@@ -144,8 +146,8 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
         if row_splits.dtype != torch.int64 or row_splits.dim() != 1 or row_splits.numel() < 1 or row_splits.device != x.device:
             raise ValueError(f"{what}: row_splits must be a non-empty 1-d int64 tensor on {x.device}")
         row_splits = row_splits.contiguous()
-    if x.shape[-2] > _MAX_STEPS or (not packed and x.shape[0] > _MAX_STEPS) or x.shape[-1] > _MAX_STEPS:
-        raise ValueError(f"{what}: an axis is longer than {_MAX_STEPS}")
+    if x.shape[-2] > _MAX_STEPS or (not packed and x.shape[0] > _MAX_STEPS) or x.shape[-1] > _MAX_CHANNELS:
+        raise ValueError(f"{what}: more than {_MAX_STEPS} steps or sequences, or than {_MAX_CHANNELS} channels")
     if h0 is not None:
         _check_state(h0, (row_splits.numel() - 1 if packed else x.shape[0], x.shape[-1]), x, what, "h0")
     ops._require_cuda(gate, x)
