@@ -15,12 +15,12 @@
 // Lanes: CG channel groups of VEC adjacent channels x 64 / CG stretches; NW waves share a tile.
 //
 // A (sequence, block of channels) is a chain; its tiles follow one another.
-//   many chains (CHAIN = false): NW waves walk a whole chain (NW = 1: four independent chains a workgroup, no barrier);
+//   many chains (CHAIN = false): a wave walks a whole chain, four independent ones a workgroup, no barrier;
 //   few chains (CHAIN = true): a workgroup takes ONE tile.  It publishes the tile's (P, H), collects those of the tiles in front of it and goes on
 //     with the state they make: every tensor is still read and written once.  The collection has a fixed shape, whatever the order of
 //     arrival: tiles in groups of 16, groups in sets of 16; a group's last tile publishes the group's (P, H), a set's last tile the state behind it;
 //     a tile composes the set's state, the groups of its set and the tiles of its group in front of it, at most 31 entries.
-//     Tiles are handed out by a counter, those of every chain in order, so a tile waits only for workgroups that already run (each
+//     Tiles are handed out by a counter per chain, in order, so a tile waits only for workgroups that already run (each
 //     publishes its own (P, H) before it waits for anything), and every wait ends.  An entry is one 64-bit word, written and read
 //     by relaxed device-scope atomics: it is there or it is not, no fence is needed.  The words are set to "empty" by a launch in front.
 #pragma once
@@ -31,6 +31,7 @@
 #define NF_SCAN_MAX_CHANNELS (1 << 20)
 #define NF_SCAN_FAN 16                               // tiles a group, groups a set
 #define NF_SCAN_EMPTY 0xffffffffffffffffull
+#define NF_SCAN_LINE 32                              // ints between two chains' counters: a cache line (one counter for all took 15 ns a tile)
 #define NF_SCAN_CLOSED 0xfffffffeu                   // in P's place: a sequence begins inside, nothing of the entering state comes out
 
 struct NfScanArgs {
@@ -76,78 +77,78 @@ template <typename E, int VEC, int TPT> struct NfStretch {
     {
         typedef typename NfVec<E, VEC>::type V;
         if (rows.last == TS - 1) {
-            const unsigned o = rows.at(jl) * (unsigned)step + lane_off;
+            unsigned o = rows.at(jl) * (unsigned)step + lane_off;
             const int s = rows.rev ? -step : step;
 #pragma unroll
-            for (int i = 0; i < TPT; ++i) r[i] = *(const V*)(base + (unsigned)(o + i * s));
+            for (int i = 0; i < TPT; ++i) { r[i] = *(const V*)(base + o); o += s; }
         } else {
 #pragma unroll
             for (int i = 0; i < TPT; ++i) r[i] = *(const V*)(base + (unsigned)(rows.at(min(jl + i, rows.last)) * (unsigned)step + lane_off));
         }
     }
+    __device__ __forceinline__ void clear(unsigned idle)
+    {
+#pragma unroll
+        for (int i = 0; i < TPT; ++i)
+            if (idle >> i & 1u)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) r[i][k] = 0;
+    }
     __device__ __forceinline__ float at(int i, int k) const { return E::cv(r[i][k]); }
 };
 
-// The gate comes in the storage type or in fp32, per channel or one per step: both are uniform branches.
-template <typename E, int VEC, int TPT> struct NfGateStretch {
-    unsigned r[TPT * VEC];               // fp32: a word per channel; else the row's VEC elements packed from word VEC * i on
-    template <typename W, int TS>
-    __device__ __forceinline__ void load_as(const char* base, unsigned lane_off, int step, int jl, const NfRows<TS>& rows)
-    {
-        constexpr int N = (sizeof(W) + 3) / 4;
-        const bool full = rows.last == TS - 1;
-        const unsigned o = rows.at(jl) * (unsigned)step + lane_off;
-        const int s = rows.rev ? -step : step;
+// The gate as factors.  It comes in the storage type or in fp32 (a uniform branch), per channel or one per step (SHARED).
+template <typename W, int N, int TPT, int TS>
+__device__ __forceinline__ void nf_gate_words(unsigned (&r)[TPT][N], const char* base, unsigned lane_off, int step, int jl, const NfRows<TS>& rows)
+{
+    const bool full = rows.last == TS - 1;
+    unsigned o = rows.at(jl) * (unsigned)step + lane_off;
+    const int s = rows.rev ? -step : step;
 #pragma unroll
-        for (int i = 0; i < TPT; ++i) {
-            const unsigned oo = full ? (unsigned)(o + i * s) : rows.at(min(jl + i, rows.last)) * (unsigned)step + lane_off;
-            const W v = *(const W*)(base + oo);
-            if constexpr (sizeof(W) < 4) r[VEC * i] = (unsigned)v;
-            else if constexpr (N == 1) r[VEC * i] = __builtin_bit_cast(unsigned, v);
-            else
+    for (int i = 0; i < TPT; ++i) {
+        const W v = *(const W*)(base + (full ? o : (unsigned)(rows.at(min(jl + i, rows.last)) * (unsigned)step + lane_off)));
+        o += s;
+        if constexpr (sizeof(W) < 4) r[i][0] = (unsigned)v;
+        else if constexpr (sizeof(W) == 4) r[i][0] = __builtin_bit_cast(unsigned, v);
+        else
 #pragma unroll
-                for (int k = 0; k < N; ++k) r[VEC * i + k] = v[k];
-        }
+            for (int k = 0; k < (int)(sizeof(W) / 4); ++k) r[i][k] = v[k];
     }
+}
+template <typename E, int VEC, int TPT, bool SHARED> struct NfGateStretch {
+    static constexpr int N = SHARED ? 1 : VEC;
+    unsigned r[TPT][N];                  // fp32: a word per channel; else packed from word 0 on
     template <int TS> __device__ __forceinline__ void load(const NfScanArgs& a, const char* base, unsigned lane_off, int jl, const NfRows<TS>& rows)
     {
-        typedef unsigned W32 __attribute__((ext_vector_type(VEC)));
-        typedef unsigned W16 __attribute__((ext_vector_type(VEC >= 4 ? VEC / 2 : 2)));
+        typedef unsigned W32 __attribute__((ext_vector_type(N >= 2 ? N : 2)));
+        typedef unsigned W16 __attribute__((ext_vector_type(N >= 4 ? N / 2 : 2)));
         if (sizeof(typename E::st) == 4 || a.gate32) {
-            if (a.shared || VEC == 1) load_as<unsigned>(base, lane_off, a.gate_st, jl, rows);
-            else load_as<W32>(base, lane_off, a.gate_st, jl, rows);
+            if constexpr (N == 1) nf_gate_words<unsigned>(r, base, lane_off, a.gate_st, jl, rows);
+            else nf_gate_words<W32>(r, base, lane_off, a.gate_st, jl, rows);
         } else {
-            if (a.shared || VEC == 1) load_as<unsigned short>(base, lane_off, a.gate_st, jl, rows);
-            else if (VEC == 2) load_as<unsigned>(base, lane_off, a.gate_st, jl, rows);
-            else load_as<W16>(base, lane_off, a.gate_st, jl, rows);
+            if constexpr (N == 1) nf_gate_words<unsigned short>(r, base, lane_off, a.gate_st, jl, rows);
+            else if constexpr (N == 2) nf_gate_words<unsigned>(r, base, lane_off, a.gate_st, jl, rows);
+            else nf_gate_words<W16>(r, base, lane_off, a.gate_st, jl, rows);
         }
     }
-    __device__ __forceinline__ void get(const NfScanArgs& a, float (&A)[TPT][VEC]) const
+    __device__ __forceinline__ void get(const NfScanArgs& a, float (&A)[TPT][N]) const
     {
+        if (sizeof(typename E::st) == 4 || a.gate32) {
 #pragma unroll
-        for (int i = 0; i < TPT; ++i) {
-            if (sizeof(typename E::st) == 4 || a.gate32) {
+            for (int i = 0; i < TPT; ++i)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) A[i][k] = __uint_as_float(r[VEC * i + (a.shared ? 0 : k)]);
-            } else {
+                for (int k = 0; k < N; ++k) A[i][k] = __uint_as_float(r[i][k]);
+        } else {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const unsigned w = r[VEC * i + (a.shared ? 0 : k / 2)];
-                    A[i][k] = E::cv((typename E::st)((k & 1) && !a.shared ? w >> 16 : w & 0xffffu));
-                }
-            }
+            for (int i = 0; i < TPT; ++i)
+#pragma unroll
+                for (int k = 0; k < N; ++k) A[i][k] = E::cv((typename E::st)((k & 1) ? r[i][k / 2] >> 16 : r[i][k / 2] & 0xffffu));
         }
         if (a.log_gate) {
 #pragma unroll
-            for (int i = 0; i < TPT; ++i) {
-                if (a.shared) {
-                    const float e = expf(A[i][0]);
+            for (int i = 0; i < TPT; ++i)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) A[i][k] = e;
-                } else
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) A[i][k] = expf(A[i][k]);
-            }
+                for (int k = 0; k < N; ++k) A[i][k] = expf(A[i][k]);
         }
     }
 };
@@ -180,318 +181,396 @@ template <int TPT> __device__ __forceinline__ NfMarks nf_scan_marks(const int* s
     return m;
 }
 
-template <int VEC> struct NfAgg {
-    float P[VEC], H[VEC];
+// (P, H) of a stretch: N products (1: one gate for all channels), VEC states.
+template <int VEC, int N, bool PACKED> struct NfAgg {
+    float P[N], H[VEC];
     int closed;             // a sequence begins inside: nothing of the entering state comes out
+    __device__ __forceinline__ bool shut() const { return PACKED && closed; }
     __device__ __forceinline__ void after(const NfAgg& p)      // this stretch behind stretch p
     {
-        if (closed) return;
+        if (shut()) return;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) { H[k] = fmaf(P[k], p.H[k], H[k]); P[k] *= p.P[k]; }
-        closed = p.closed;
+        for (int k = 0; k < VEC; ++k) H[k] = fmaf(P[N == 1 ? 0 : k], p.H[k], H[k]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) P[k] *= p.P[k];
+        if (PACKED) closed = p.closed;
     }
     __device__ __forceinline__ void apply(float (&c)[VEC]) const
     {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) c[k] = closed ? H[k] : fmaf(P[k], c[k], H[k]);
+        for (int k = 0; k < VEC; ++k) c[k] = shut() ? H[k] : fmaf(P[N == 1 ? 0 : k], c[k], H[k]);
     }
     __device__ __forceinline__ void one()
     {
         closed = 0;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) { P[k] = 1.f; H[k] = 0.f; }
+        for (int k = 0; k < N; ++k) P[k] = 1.f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) H[k] = 0.f;
     }
 };
 
-// Composition over the stretches of a wave in processing order (DIR = 0: upwards, 1: downwards): `a` becomes the composition of
-// everything in front of this lane's stretch, `total` that of the whole wave (in every lane).
-template <int VEC, int CG, int DIR> __device__ __forceinline__ void nf_wave_scan(NfAgg<VEC>& a, NfAgg<VEC>& total, int tg, int packed)
+// f(value) for every value of a stretch that lanes exchange
+template <int VEC, int N, bool PACKED, typename F> __device__ __forceinline__ NfAgg<VEC, N, PACKED> nf_map(const NfAgg<VEC, N, PACKED>& a, F f)
 {
-    constexpr int TG = 64 / CG;
-    auto shift = [&](float v, int d) { return DIR ? __shfl_down(v, d) : __shfl_up(v, d); };
-    auto shifti = [&](int v, int d) { return DIR ? __shfl_down(v, d) : __shfl_up(v, d); };
-    const int pos = DIR ? TG - 1 - tg : tg;
+    NfAgg<VEC, N, PACKED> r;
 #pragma unroll
-    for (int s = 1; s < TG; s *= 2) {
-        NfAgg<VEC> p;
+    for (int k = 0; k < N; ++k) r.P[k] = __int_as_float(f(__float_as_int(a.P[k])));
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) { p.P[k] = shift(a.P[k], s * CG); p.H[k] = shift(a.H[k], s * CG); }
-        p.closed = packed ? shifti(a.closed, s * CG) : 0;
-        if (pos >= s) a.after(p);
-    }
-    const int cg = (threadIdx.x & 63) % CG, last = (DIR ? 0 : TG - 1) * CG + cg;
-    total.closed = packed ? __shfl(a.closed, last) : 0;
+    for (int k = 0; k < VEC; ++k) r.H[k] = __int_as_float(f(__float_as_int(a.H[k])));
+    r.closed = PACKED ? f(a.closed) : 0;
+    return r;
+}
+template <int VEC, int N, bool PACKED> __device__ __forceinline__ void nf_take(NfAgg<VEC, N, PACKED>& a, bool take, const NfAgg<VEC, N, PACKED>& b)
+{
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) { total.P[k] = __shfl(a.P[k], last); total.H[k] = __shfl(a.H[k], last); }
-    NfAgg<VEC> e;
+    for (int k = 0; k < N; ++k) a.P[k] = take ? b.P[k] : a.P[k];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) { e.P[k] = shift(a.P[k], CG); e.H[k] = shift(a.H[k], CG); }
-    e.closed = packed ? shifti(a.closed, CG) : 0;
-    if (pos == 0) e.one();
-    a = e;
+    for (int k = 0; k < VEC; ++k) a.H[k] = take ? b.H[k] : a.H[k];
+    if (PACKED) a.closed = take ? b.closed : a.closed;
 }
 
-// LDS exchange of the waves' totals; two buffers, so that one barrier a tile is enough (a wave can be at most one tile ahead).
-template <int VEC, int CG, int NW> struct NfScanLds {
-    float P[2][NW][CG * VEC], H[2][NW][CG * VEC];
-    int closed[2][NW];
-    __device__ __forceinline__ void put(int buf, int w, int lane, const NfAgg<VEC>& t)
+// Composition over the stretches of a wave in processing order (DIR = 0: upwards, 1: downwards): `a` becomes the composition of
+// everything in front of this lane's stretch, `total` that of the whole wave (in every lane).
+template <int CG, int DIR, int VEC, int N, bool PACKED>
+__device__ __forceinline__ void nf_wave_scan(NfAgg<VEC, N, PACKED>& a, NfAgg<VEC, N, PACKED>& total, int tg)
+{
+    typedef NfAgg<VEC, N, PACKED> Agg;
+    constexpr int TG = 64 / CG;
+    const int lane = threadIdx.x & 63;
+    if constexpr (TG == 4) {
+        // four rows of 16 lanes: the row exchanges of the vector unit (no trip through LDS).  Pairs of rows, then halves.
+        auto lo16 = [](int v) { return (int)__builtin_amdgcn_permlane16_swap(v, v, false, false)[0]; };       // rows 0 0 2 2
+        auto hi16 = [](int v) { return (int)__builtin_amdgcn_permlane16_swap(v, v, false, false)[1]; };       // rows 1 1 3 3
+        auto lo32 = [](int v) { return (int)__builtin_amdgcn_permlane32_swap(v, v, false, false)[0]; };
+        auto hi32 = [](int v) { return (int)__builtin_amdgcn_permlane32_swap(v, v, false, false)[1]; };
+        const Agg even = nf_map(a, lo16), odd = nf_map(a, hi16);
+        const Agg first = DIR ? odd : even;
+        Agg pair = DIR ? even : odd;
+        pair.after(first);
+        const Agg low = nf_map(pair, lo32), high = nf_map(pair, hi32);
+        const Agg half = DIR ? high : low;
+        total = DIR ? low : high;
+        total.after(half);
+        a.one();
+        nf_take(a, ((tg & 1) != 0) != (DIR != 0), first);       // the second row of a pair
+        Agg e = a;
+        e.after(half);
+        nf_take(a, (tg >= 2) != (DIR != 0), e);                 // the second half
+    } else {
+        const int pos = DIR ? TG - 1 - tg : tg;
+        auto from = [](int v, int l) { return __builtin_amdgcn_ds_bpermute(4 * l, v); };
+#pragma unroll
+        for (int s = 1; s < TG; s *= 2) {
+            const int l = lane + (DIR ? s * CG : -s * CG);
+            const Agg p = nf_map(a, [&](int v) { return from(v, l); });
+            if (pos >= s) a.after(p);
+        }
+        const int last = (DIR ? 0 : TG - 1) * CG + lane % CG;
+        total = nf_map(a, [&](int v) { return from(v, last); });
+        const int l = lane + (DIR ? CG : -CG);
+        a = nf_map(a, [&](int v) { return from(v, l); });
+        Agg e;
+        e.one();
+        nf_take(a, pos == 0, e);
+    }
+}
+
+// LDS exchange of the waves' totals
+template <int VEC, int N, int CG, int NW, bool PACKED> struct NfScanLds {
+    typedef NfAgg<VEC, N, PACKED> Agg;
+    float P[NW][CG * N], H[NW][CG * VEC];
+    int closed[NW];
+    __device__ __forceinline__ void put(int w, int lane, const Agg& t)
     {
         if (lane < CG) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) { P[buf][w][lane * VEC + k] = t.P[k]; H[buf][w][lane * VEC + k] = t.H[k]; }
-            if (lane == 0) closed[buf][w] = t.closed;
+            for (int k = 0; k < N; ++k) P[w][lane * N + k] = t.P[k];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) H[w][lane * VEC + k] = t.H[k];
+            if (PACKED && lane == 0) closed[w] = t.closed;
         }
     }
-    __device__ __forceinline__ NfAgg<VEC> get(int buf, int w, int cg) const
+    __device__ __forceinline__ Agg get(int w, int cg) const
     {
-        NfAgg<VEC> t;
+        Agg t;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) { t.P[k] = P[buf][w][cg * VEC + k]; t.H[k] = H[buf][w][cg * VEC + k]; }
-        t.closed = closed[buf][w];
+        for (int k = 0; k < N; ++k) t.P[k] = P[w][cg * N + k];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) t.H[k] = H[w][cg * VEC + k];
+        t.closed = PACKED ? closed[w] : 0;
         return t;
     }
 };
 
 // ---- the chain's exchange --------------------------------------------------------------------------
-template <int VEC> __device__ __forceinline__ void nf_publish(unsigned long long* p, const NfAgg<VEC>& t)
+template <int VEC, int N, bool PACKED> __device__ __forceinline__ void nf_publish(unsigned long long* p, const NfAgg<VEC, N, PACKED>& t)
 {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-        const unsigned P = t.closed ? NF_SCAN_CLOSED : t.P[k] != t.P[k] ? 0x7fc00000u : __float_as_uint(t.P[k]);      // (a NaN never looks like a mark)
+        const float f = t.P[N == 1 ? 0 : k];
+        const unsigned P = t.shut() ? NF_SCAN_CLOSED : f != f ? 0x7fc00000u : __float_as_uint(f);      // (a NaN never looks like a mark)
         __hip_atomic_store(p + k, (unsigned long long)__float_as_uint(t.H[k]) << 32 | P, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
-template <int VEC> struct NfEntry {
+template <int VEC, int N, bool PACKED> struct NfEntry {
     unsigned long long w[VEC];
     __device__ __forceinline__ void ask(const unsigned long long* p)
     {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) w[k] = __hip_atomic_load(p + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __device__ __forceinline__ NfAgg<VEC> wait(const unsigned long long* p)
+    __device__ __forceinline__ bool missing() const
     {
-        NfAgg<VEC> t;
+        bool m = false;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m |= w[k] == NF_SCAN_EMPTY;
+        return m;
+    }
+    __device__ __forceinline__ NfAgg<VEC, N, PACKED> wait(const unsigned long long* p)
+    {
+        while (missing()) { __builtin_amdgcn_s_sleep(2); ask(p); }      // (a pause: the polls go past the caches)
+        NfAgg<VEC, N, PACKED> t;
         t.closed = 0;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            while (w[k] == NF_SCAN_EMPTY) w[k] = __hip_atomic_load(p + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            t.P[k] = __uint_as_float((unsigned)w[k]); t.H[k] = __uint_as_float((unsigned)(w[k] >> 32));
-            t.closed |= (unsigned)w[k] == NF_SCAN_CLOSED;
-        }
+        for (int k = 0; k < N; ++k) t.P[k] = __uint_as_float((unsigned)w[k]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) t.H[k] = __uint_as_float((unsigned)(w[k] >> 32));
+        if (PACKED) t.closed = (unsigned)w[0] == NF_SCAN_CLOSED;
         return t;
     }
 };
 
-// The state that enters tile k of a chain (one wave's work; c = the chain's initial state), and the publications that tile k owes: `own` is its (P, H).
-template <int VEC, int CG> __device__ __forceinline__ void nf_chain(const NfScanArgs& a, int k, int chain, int nchains, int cg, int tg,
-                                                                    const NfAgg<VEC>& own, int packed, float (&c)[VEC])
+// What enters tile k of a chain, collected by two waves (role 0: the tiles of k's group in front of it, and the publications that tile k owes,
+// `own` being its (P, H); role 1: the groups of its set, and the set's state), left in LDS.
+template <int VEC, int N, int CG, bool PACKED> struct NfChainLds {
+    NfScanLds<VEC, N, CG, 2, PACKED> part;
+    float set[CG * VEC];
+};
+template <int VEC, int CG> __device__ __forceinline__ unsigned long long* nf_chain_word(const NfScanArgs& a, unsigned long long* ws, int idx, int chain, int cg)
 {
-    constexpr int TG = 64 / CG, CH = CG * VEC, PER = (NF_SCAN_FAN - 1 + TG - 1) / TG;
+    return ws + ((long long)idx * (a.B * a.nblk) + chain) * (CG * VEC) + cg * VEC;
+}
+template <int VEC, int N, int CG, bool PACKED>
+__device__ __forceinline__ void nf_chain_collect(const NfScanArgs& a, int role, int k, int chain, int cg, int tg, const NfAgg<VEC, N, PACKED>& own,
+                                                 NfChainLds<VEC, N, CG, PACKED>& lds)
+{
+    constexpr int TG = 64 / CG, PER = (NF_SCAN_FAN - 1 + TG - 1) / TG;
     const int grp = k / NF_SCAN_FAN, set = grp / NF_SCAN_FAN, nt = k % NF_SCAN_FAN, ng = grp % NF_SCAN_FAN;
-    auto word = [&](unsigned long long* ws, int idx) { return ws + ((long long)idx * nchains + chain) * CH + cg * VEC; };
-    if (k + 1 < a.ntiles && tg == 0) nf_publish<VEC>(word(a.ws_tile, k), own);
-    NfEntry<VEC> et[PER], eg[PER], es;
+    if (role == 0 && k + 1 < a.ntiles && tg == 0) nf_publish(nf_chain_word<VEC, CG>(a, a.ws_tile, k, chain, cg), own);
+    const int n = role == 0 ? nt : ng, first = role == 0 ? grp * NF_SCAN_FAN : set * NF_SCAN_FAN;
+    unsigned long long* ws = role == 0 ? a.ws_tile : a.ws_group;
+    NfEntry<VEC, N, PACKED> et[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = tg * PER + i;
-        if (e < nt) et[i].ask(word(a.ws_tile, grp * NF_SCAN_FAN + e));
-        if (e < ng) eg[i].ask(word(a.ws_group, set * NF_SCAN_FAN + e));
-    }
-    if (set > 0) es.ask(word(a.ws_set, set - 1));
-    NfAgg<VEC> t, tot;
+    for (int i = 0; i < PER; ++i)
+        if (tg * PER + i < n) et[i].ask(nf_chain_word<VEC, CG>(a, ws, first + tg * PER + i, chain, cg));
+    NfAgg<VEC, N, PACKED> t, tot;
     t.one();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = tg * PER + i;
-        if (e < nt) { NfAgg<VEC> n = et[i].wait(word(a.ws_tile, grp * NF_SCAN_FAN + e)); if (i > 0) n.after(t); t = n; }
+    for (int i = 0; i < PER; ++i)
+        if (tg * PER + i < n) {
+            NfAgg<VEC, N, PACKED> e = et[i].wait(nf_chain_word<VEC, CG>(a, ws, first + tg * PER + i, chain, cg));
+            if (i > 0) e.after(t);
+            t = e;
+        }
+    nf_wave_scan<CG, 0>(t, tot, tg);
+    if (role == 0 && nt == NF_SCAN_FAN - 1 && k + 1 < a.ntiles && tg == 0) {
+        NfAgg<VEC, N, PACKED> g = own;
+        g.after(tot);
+        nf_publish(nf_chain_word<VEC, CG>(a, a.ws_group, grp, chain, cg), g);
     }
-    nf_wave_scan<VEC, CG, 0>(t, tot, tg, packed);
-    const NfAgg<VEC> tiles = tot;
-    if (nt == NF_SCAN_FAN - 1 && k + 1 < a.ntiles && tg == 0) {
-        NfAgg<VEC> g = own;
-        g.after(tiles);
-        nf_publish<VEC>(word(a.ws_group, grp), g);
-    }
-    t.one();
+    lds.part.put(role, threadIdx.x & 63, tot);
+    if (tg == 0 && role == 1 && set > 0) {
+        const unsigned long long* p = nf_chain_word<VEC, CG>(a, a.ws_set, set - 1, chain, cg);
+        NfEntry<VEC, N, PACKED> e;
+        e.ask(p);
+        const NfAgg<VEC, N, PACKED> s = e.wait(p);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = tg * PER + i;
-        if (e < ng) { NfAgg<VEC> n = eg[i].wait(word(a.ws_group, set * NF_SCAN_FAN + e)); if (i > 0) n.after(t); t = n; }
+        for (int i = 0; i < VEC; ++i) lds.set[cg * VEC + i] = s.H[i];
     }
-    nf_wave_scan<VEC, CG, 0>(t, tot, tg, packed);
-    if (set > 0) {
-        const NfAgg<VEC> s = es.wait(word(a.ws_set, set - 1));
+}
+// Behind a barrier: c becomes the state that enters tile k; a set's last tile publishes the state behind it.
+template <int VEC, int N, int CG, bool PACKED>
+__device__ __forceinline__ void nf_chain_enter(const NfScanArgs& a, int k, int chain, int cg, bool publisher, const NfAgg<VEC, N, PACKED>& own,
+                                               const NfChainLds<VEC, N, CG, PACKED>& lds, float (&c)[VEC])
+{
+    const int set = k / (NF_SCAN_FAN * NF_SCAN_FAN);
+    if (set > 0)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) c[i] = s.H[i];
-    }
-    tot.apply(c);
-    tiles.apply(c);
-    if (nt == NF_SCAN_FAN - 1 && ng == NF_SCAN_FAN - 1 && k + 1 < a.ntiles && tg == 0) {
-        float o[VEC];
-        NfAgg<VEC> s;
+        for (int i = 0; i < VEC; ++i) c[i] = lds.set[cg * VEC + i];
+    lds.part.get(1, cg).apply(c);
+    lds.part.get(0, cg).apply(c);
+    if (publisher && (k + 1) % (NF_SCAN_FAN * NF_SCAN_FAN) == 0 && k + 1 < a.ntiles) {
+        NfAgg<VEC, N, PACKED> s;
         s.one();
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = c[i];
-        own.apply(o);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) s.H[i] = o[i];
-        nf_publish<VEC>(word(a.ws_set, set), s);
+        for (int i = 0; i < VEC; ++i) s.H[i] = c[i];
+        own.apply(s.H);
+        nf_publish(nf_chain_word<VEC, CG>(a, a.ws_set, set, chain, cg), s);
     }
 }
 
-// A workgroup's place: the chain, and for CHAIN its tile by ticket.
-struct NfPlace { int blk, b, k, w; bool ok; };
-template <int NW, bool CHAIN> __device__ __forceinline__ NfPlace nf_place(const NfScanArgs& a)
+// A wave's place: its chain, and for CHAIN the workgroup's tile by ticket.
+struct NfPlace { int blk, b, k, w, chain; bool ok; };
+template <bool CHAIN> __device__ __forceinline__ NfPlace nf_place(const NfScanArgs& a)
 {
     __shared__ int s_ticket;
     NfPlace p;
     const int nchains = a.B * a.nblk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int chain;
     if (CHAIN) {
-        if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        p.chain = blockIdx.x % nchains;
+        if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(a.ticket + p.chain * NF_SCAN_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        const int t = __builtin_amdgcn_readfirstlane(s_ticket);
-        chain = t % nchains;
-        p.k = t / nchains;
+        p.k = __builtin_amdgcn_readfirstlane(s_ticket);
+        p.w = wave;
     } else {
-        chain = NW == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
-        p.k = 0;
+        p.chain = blockIdx.x * (NF_SCAN_WG / 64) + wave;
+        p.k = p.w = 0;
     }
-    p.ok = chain < nchains;
-    p.blk = chain % a.nblk;
-    p.b = chain / a.nblk;
-    p.w = NW == 1 ? 0 : wave;
+    p.ok = p.chain < nchains;
+    p.blk = p.chain % a.nblk;
+    p.b = p.chain / a.nblk;
     return p;
 }
+
+// Steps of a stretch that are not the tensor's (bit i).
+template <int TPT> __device__ __forceinline__ unsigned nf_beyond(int j0, int T) { return j0 + TPT <= T ? 0u : j0 >= T ? ~0u : ~0u << (T - j0); }
 
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN>
-__global__ void __launch_bounds__(NW == 1 ? NF_SCAN_WG : 64 * NW) k_scan_fwd(NfScanArgs a)
+template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN, bool PACKED, bool SHARED>
+__global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_fwd(NfScanArgs a)
 {
-    constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st);
-    __shared__ NfScanLds<VEC, CG, NW> lds;
-    __shared__ float s_c[CHAIN ? CG * VEC : 1];
-    const NfPlace pl = nf_place<NW, CHAIN>(a);
-    if (!pl.ok) return;                                  // (NW = 1 only: no barrier below)
+    constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st), N = SHARED ? 1 : VEC;
+    typedef NfAgg<VEC, N, PACKED> Agg;
+    __shared__ NfScanLds<VEC, N, CG, CHAIN ? NW : 1, PACKED> lds;
+    __shared__ NfChainLds<VEC, N, CG, PACKED> s_chain;
+    const NfPlace pl = nf_place<CHAIN>(a);
+    if (!pl.ok) return;                                  // (whole chains by waves only: no barrier below)
     const int lane = threadIdx.x & 63, cg = lane % CG, tg = lane / CG, w = pl.w, b = pl.b;
     const int ch = (pl.blk * CG + cg) * VEC;
     const bool live = ch < a.D;
     const int chl = live ? ch : 0;
-    const int T = a.T, rev = a.reverse, packed = a.sid != nullptr;
+    const int T = a.T, rev = a.reverse;
     const int gs = (ES == 4 || a.gate32) ? 4 : 2, hstep = a.D * ES;
     const char* gbase = (const char*)a.gate + b * a.gate_sb;
     const char* xbase = (const char*)a.x + b * a.x_sb;
     char* hbase = (char*)a.h + (long long)b * T * hstep;
-    const unsigned goff = a.shared ? 0u : (unsigned)(chl * gs), xoff = (unsigned)(chl * ES);
+    const unsigned goff = SHARED ? 0u : (unsigned)(chl * gs), xoff = (unsigned)(chl * ES);
     const int jl = (w * TG + tg) * TPT;
     float c[VEC];                        // the state that enters the tile
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) c[k] = (a.h0 && !packed) ? a.h0[(long long)b * a.D + chl + k] : 0.f;
-    int buf = 0;
-    for (int tile = pl.k; tile < (CHAIN ? pl.k + 1 : a.ntiles); ++tile, buf ^= 1) {
+    for (int k = 0; k < VEC; ++k) c[k] = 0.f;
+    if (a.h0 && !PACKED)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) c[k] = a.h0[(long long)b * a.D + chl + k];
+    auto initial = [&](int j, float (&s)[VEC]) {         // the state in front of step j, the first of its sequence
+        const int q = a.sid[rev ? T - 1 - j : j];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s[k] = a.h0 ? a.h0[(long long)q * a.D + chl + k] : 0.f;
+    };
+    for (int tile = pl.k; tile < (CHAIN ? pl.k + 1 : a.ntiles); ++tile) {
         const NfRows<TS> rows(tile, T, rev);
         const long long row0 = rows.first(tile, T);
-        NfStretch<E, VEC, TPT> xs;
-        NfGateStretch<E, VEC, TPT> gt;
+        NfStretch<E, VEC, TPT> x;
+        NfGateStretch<E, VEC, TPT, SHARED> gt;
         gt.load(a, gbase + row0 * a.gate_st, goff, jl, rows);
-        xs.load(xbase + row0 * a.x_st, xoff, a.x_st, jl, rows);
+        x.load(xbase + row0 * a.x_st, xoff, a.x_st, jl, rows);
         const int j0 = tile * TS + jl;
+        const bool edge = tile == a.ntiles - 1;          // (uniform) the last tile: steps that do not exist, the final state
         NfMarks m = {0u, 0u, 0u};
-        if (packed) m = nf_scan_marks<TPT>(a.sid, j0, T, rev);
-        else if (j0 < T && j0 + TPT >= T) m.end = 1u << (T - 1 - j0);
-        float A[TPT][VEC], x[TPT][VEC];
+        if (PACKED) m = nf_scan_marks<TPT>(a.sid, j0, T, rev);
+        float A[TPT][N];
         gt.get(a, A);
-#pragma unroll
-        for (int i = 0; i < TPT; ++i)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) x[i][k] = xs.at(i, k);
-        unsigned idle = m.none;
-        if (j0 + TPT > T) idle |= j0 >= T ? ~0u : ~0u << (T - j0);
-        if (idle) {
+        if (PACKED || edge) {
+            const unsigned idle = m.none | nf_beyond<TPT>(j0, T);
+            x.clear(idle);
 #pragma unroll
             for (int i = 0; i < TPT; ++i)
                 if (idle >> i & 1u)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) { A[i][k] = 1.f; x[i][k] = 0.f; }
+                    for (int k = 0; k < N; ++k) A[i][k] = 1.f;
         }
-        if (packed && m.start && a.h0) { // the first step of a sequence: its initial state goes in with x, nothing comes from before
-#pragma unroll
-            for (int i = 0; i < TPT; ++i)
-                if (m.start >> i & 1u) {
-                    const int s = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) x[i][k] = fmaf(A[i][k], a.h0[(long long)s * a.D + chl + k], x[i][k]);
-                }
-        }
-        NfAgg<VEC> me, tot;
+        Agg me, tot;
         me.one();
-        if (packed && m.start) {
+        if (PACKED && m.start) {
             me.closed = 1;
 #pragma unroll
-            for (int i = 0; i < TPT; ++i)
+            for (int i = 0; i < TPT; ++i) {
+                if (m.start >> i & 1u) initial(j0 + i, me.H);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) me.H[k] = (m.start >> i & 1u) ? x[i][k] : fmaf(A[i][k], me.H[k], x[i][k]);
+                for (int k = 0; k < VEC; ++k) me.H[k] = fmaf(A[i][N == 1 ? 0 : k], me.H[k], x.at(i, k));
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < TPT; ++i)
+            for (int i = 0; i < TPT; ++i) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) { me.H[k] = fmaf(A[i][k], me.H[k], x[i][k]); me.P[k] *= A[i][k]; }
-        }
-        nf_wave_scan<VEC, CG, 0>(me, tot, tg, packed);
-        if (NW > 1) {
-            lds.put(buf, w, lane, tot);
-            __syncthreads();
-        }
-        if (CHAIN) {
-            if (w == 0) {
-                NfAgg<VEC> own = lds.get(buf, 0, cg);
+                for (int k = 0; k < VEC; ++k) me.H[k] = fmaf(A[i][N == 1 ? 0 : k], me.H[k], x.at(i, k));
 #pragma unroll
-                for (int v = 1; v < NW; ++v) { NfAgg<VEC> n = lds.get(buf, v, cg); n.after(own); own = n; }
-                nf_chain<VEC, CG>(a, tile, pl.b * a.nblk + pl.blk, a.B * a.nblk, cg, tg, own, packed, c);
-                if (tg == 0)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) s_c[cg * VEC + k] = c[k];
+                for (int k = 0; k < N; ++k) me.P[k] *= A[i][k];
             }
+        }
+        nf_wave_scan<CG, 0>(me, tot, tg);
+        float s[VEC];
+        if constexpr (CHAIN) {
+            lds.put(w, lane, tot);
             __syncthreads();
+            Agg own;
+            if (w == 0) {
+                own = lds.get(0, cg);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) c[k] = s_c[cg * VEC + k];
+                for (int v = 1; v < NW; ++v) { Agg n = lds.get(v, cg); n.after(own); own = n; }
+            }
+            if (w < 2) nf_chain_collect<VEC, N, CG, PACKED>(a, w, tile, pl.chain, cg, tg, own, s_chain);
+            __syncthreads();
+            nf_chain_enter<VEC, N, CG, PACKED>(a, tile, pl.chain, cg, w == 0 && tg == 0, own, s_chain, c);
         }
         if (a.states && w == 0 && tg == 0 && live)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) a.states[((long long)b * a.ntiles + tile) * a.D + ch + k] = c[k];
-        float s[VEC];
+        if constexpr (CHAIN) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) s[k] = c[k];
-        if (NW > 1) {
+            for (int v = 0; v < NW - 1; ++v)
+                if (v < w) lds.get(v, cg).apply(c);
 #pragma unroll
-            for (int v = 0; v < NW; ++v) {
-                if (v == w)
+            for (int k = 0; k < VEC; ++k) s[k] = c[k];
+        } else {
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) s[k] = c[k];
-                if (!CHAIN || v < w) lds.get(buf, v, cg).apply(c);
-            }
-        } else tot.apply(c);
+            for (int k = 0; k < VEC; ++k) s[k] = c[k];
+            tot.apply(c);
+        }
         me.apply(s);
-        if (j0 < T) {
-            char* hb = hbase + row0 * hstep;
+        char* hb = hbase + row0 * hstep;
+        unsigned ho = rows.at(jl) * (unsigned)hstep + xoff;
+        const int hs = rev ? -hstep : hstep;
+        if (!PACKED && !edge) {
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < TPT; ++i) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) s[k] = fmaf(A[i][N == 1 ? 0 : k], s[k], x.at(i, k));
+                    nf_put<E, VEC>(hb + ho, s);
+                    ho += hs;
+                }
+            }
+        } else if (live) {
 #pragma unroll
             for (int i = 0; i < TPT; ++i) {
+                if (PACKED && (m.start >> i & 1u)) initial(j0 + i, s);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) s[k] = (packed && (m.start >> i & 1u)) ? x[i][k] : fmaf(A[i][k], s[k], x[i][k]);
-                if (live && j0 + i < T) {
-                    char* q = hb + (unsigned)(rows.at(jl + i) * (unsigned)hstep + xoff);
-                    if (m.none >> i & 1u) { const float z[VEC] = {}; nf_put<E, VEC>(q, z); }
-                    else nf_put<E, VEC>(q, s);
-                    if (m.end >> i & 1u) {       // the final state is the last step's, to the bit
-                        const int q_ = packed ? a.sid[rev ? T - 1 - (j0 + i) : j0 + i] : b;
+                for (int k = 0; k < VEC; ++k) s[k] = fmaf(A[i][N == 1 ? 0 : k], s[k], x.at(i, k));
+                if (j0 + i < T) {
+                    if (PACKED && (m.none >> i & 1u)) { const float z[VEC] = {}; nf_put<E, VEC>(hb + ho, z); }
+                    else nf_put<E, VEC>(hb + ho, s);
+                    if (PACKED ? m.end >> i & 1u : j0 + i == T - 1) {        // the final state is the last step's, to the bit
+                        const int q = PACKED ? a.sid[rev ? T - 1 - (j0 + i) : j0 + i] : b;
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) a.h_last[(long long)q_ * a.D + ch + k] = s[k];
+                        for (int k = 0; k < VEC; ++k) a.h_last[(long long)q * a.D + ch + k] = s[k];
                     }
                 }
+                ho += hs;
             }
         }
     }
@@ -500,183 +579,166 @@ __global__ void __launch_bounds__(NW == 1 ? NF_SCAN_WG : 64 * NW) k_scan_fwd(NfS
 // ------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------
-template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN>
-__global__ void __launch_bounds__(NW == 1 ? NF_SCAN_WG : 64 * NW) k_scan_bwd(NfScanArgs a)
+template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN, bool PACKED, bool SHARED>
+__global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_bwd(NfScanArgs a)
 {
-    constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st);
-    __shared__ NfScanLds<VEC, CG, NW> lds_f, lds_r;
-    __shared__ float s_c[CHAIN ? CG * VEC : 1];
-    const NfPlace pl = nf_place<NW, CHAIN>(a);
+    constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st), N = SHARED ? 1 : VEC;
+    typedef NfAgg<VEC, N, PACKED> Agg;
+    __shared__ NfScanLds<VEC, N, CG, CHAIN ? NW : 1, PACKED> lds_f, lds_r;
+    __shared__ NfChainLds<VEC, N, CG, PACKED> s_chain;
+    const NfPlace pl = nf_place<CHAIN>(a);
     if (!pl.ok) return;
     const int lane = threadIdx.x & 63, cg = lane % CG, tg = lane / CG, w = pl.w, b = pl.b;
     const int ch = (pl.blk * CG + cg) * VEC;
     const bool live = ch < a.D;
     const int chl = live ? ch : 0;
-    const int T = a.T, rev = a.reverse, packed = a.sid != nullptr;
+    const int T = a.T, rev = a.reverse;
     const int gs = (ES == 4 || a.gate32) ? 4 : 2, hstep = a.D * ES, gstep = a.D * gs;
     const char* gbase = (const char*)a.gate + b * a.gate_sb;
     const char* xbase = (const char*)a.x + b * a.x_sb;
     const char* ybase = a.g ? (const char*)a.g + b * a.g_sb : nullptr;
-    const unsigned goff = a.shared ? 0u : (unsigned)(chl * gs), xoff = (unsigned)(chl * ES);
+    const unsigned goff = SHARED ? 0u : (unsigned)(chl * gs), xoff = (unsigned)(chl * ES);
     const int jl = (w * TG + tg) * TPT;
     float u[VEC];                        // the gradient that enters the tile from behind
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) u[k] = (a.g_last && !packed) ? a.g_last[(long long)b * a.D + chl + k] : 0.f;
-    int buf = 0;
-    for (int it = pl.k; it < (CHAIN ? pl.k + 1 : a.ntiles); ++it, buf ^= 1) {
+    for (int k = 0; k < VEC; ++k) u[k] = 0.f;
+    if (a.g_last && !PACKED)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) u[k] = a.g_last[(long long)b * a.D + chl + k];
+    auto of_sequence = [&](const float* p, int j, float (&s)[VEC]) {         // the row of p that belongs to step j's sequence, or zeros
+        const int q = a.sid[rev ? T - 1 - j : j];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s[k] = p ? p[(long long)q * a.D + chl + k] : 0.f;
+    };
+    for (int it = pl.k; it < (CHAIN ? pl.k + 1 : a.ntiles); ++it) {
         const int tile = a.ntiles - 1 - it;
         const NfRows<TS> rows(tile, T, rev);
         const long long row0 = rows.first(tile, T);
-        NfStretch<E, VEC, TPT> xs, ys;
-        NfGateStretch<E, VEC, TPT> gt;
+        NfStretch<E, VEC, TPT> x, y;
+        NfGateStretch<E, VEC, TPT, SHARED> gt;
         gt.load(a, gbase + row0 * a.gate_st, goff, jl, rows);
-        if (ybase) ys.load(ybase + row0 * a.g_st, xoff, a.g_st, jl, rows);
-        xs.load(xbase + row0 * a.x_st, xoff, a.x_st, jl, rows);
+        if (ybase) y.load(ybase + row0 * a.g_st, xoff, a.g_st, jl, rows);
+        else y.clear(~0u);
+        x.load(xbase + row0 * a.x_st, xoff, a.x_st, jl, rows);
         float c[VEC];                    // the state that enters the tile in front
 #pragma unroll
         for (int k = 0; k < VEC; ++k) c[k] = a.states[((long long)b * a.ntiles + tile) * a.D + chl + k];
         const int j0 = tile * TS + jl;
+        const bool edge = it == 0;       // (uniform) the tile with steps that do not exist
         NfMarks m = {0u, 0u, 0u};
-        if (packed) m = nf_scan_marks<TPT>(a.sid, j0, T, rev);
-        float A[TPT][VEC], x[TPT][VEC], y[TPT][VEC];
+        if (PACKED) m = nf_scan_marks<TPT>(a.sid, j0, T, rev);
+        float A[TPT][N];
         gt.get(a, A);
-#pragma unroll
-        for (int i = 0; i < TPT; ++i)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) { x[i][k] = xs.at(i, k); y[i][k] = ybase ? ys.at(i, k) : 0.f; }
-        unsigned idle = m.none;
-        if (j0 + TPT > T) idle |= j0 >= T ? ~0u : ~0u << (T - j0);
-        if (idle) {
+        if (PACKED || edge) {
+            const unsigned idle = m.none | nf_beyond<TPT>(j0, T);
+            x.clear(idle);
+            y.clear(idle);
 #pragma unroll
             for (int i = 0; i < TPT; ++i)
                 if (idle >> i & 1u)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) { A[i][k] = 1.f; x[i][k] = 0.f; y[i][k] = 0.f; }
+                    for (int k = 0; k < N; ++k) A[i][k] = 1.f;
         }
-        if (packed && m.end && a.g_last) {       // the last step of a sequence takes the gradient of its final state
-#pragma unroll
-            for (int i = 0; i < TPT; ++i)
-                if (m.end >> i & 1u) {
-                    const int s = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) y[i][k] += a.g_last[(long long)s * a.D + chl + k];
-                }
-        }
-        // backwards: the stretch as u -> P u + H
-        NfAgg<VEC> rv, rtot, fw, ftot;
+        // backwards: the stretch as u -> P u + H (what enters the last step of a sequence is the gradient of its final state)
+        Agg rv, rtot, fw, ftot;
         rv.one();
-        rv.closed = packed && m.end;
+        if (PACKED) rv.closed = m.end != 0u;
 #pragma unroll
-        for (int i = TPT - 1; i >= 0; --i)
+        for (int i = TPT - 1; i >= 0; --i) {
+            if (PACKED && (m.end >> i & 1u)) of_sequence(a.g_last, j0 + i, rv.H);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                rv.H[k] = A[i][k] * (((packed && (m.end >> i & 1u)) ? 0.f : rv.H[k]) + y[i][k]);
-                rv.P[k] *= A[i][k];
-            }
+            for (int k = 0; k < VEC; ++k) rv.H[k] = A[i][N == 1 ? 0 : k] * (rv.H[k] + y.at(i, k));
+#pragma unroll
+            for (int k = 0; k < N; ++k) rv.P[k] *= A[i][k];
+        }
         // forwards: the stretch as c -> P c + H, started anew where a sequence begins
         fw.one();
-        if (packed && m.start) {
-            fw.closed = 1;
+        if (PACKED) fw.closed = m.start != 0u;
 #pragma unroll
-            for (int i = 0; i < TPT; ++i) {
-                int s = 0;
-                if (m.start >> i & 1u) s = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
+        for (int k = 0; k < N; ++k) fw.P[k] = rv.P[k];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const float h0 = ((m.start >> i & 1u) && a.h0) ? a.h0[(long long)s * a.D + chl + k] : 0.f;
-                    fw.H[k] = fmaf(A[i][k], (m.start >> i & 1u) ? h0 : fw.H[k], x[i][k]);
-                }
-            }
-        } else {
+        for (int i = 0; i < TPT; ++i) {
+            if (PACKED && (m.start >> i & 1u)) of_sequence(a.h0, j0 + i, fw.H);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) fw.P[k] = rv.P[k];
-#pragma unroll
-            for (int i = 0; i < TPT; ++i)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) fw.H[k] = fmaf(A[i][k], fw.H[k], x[i][k]);
+            for (int k = 0; k < VEC; ++k) fw.H[k] = fmaf(A[i][N == 1 ? 0 : k], fw.H[k], x.at(i, k));
         }
-        nf_wave_scan<VEC, CG, 1>(rv, rtot, tg, packed);
-        nf_wave_scan<VEC, CG, 0>(fw, ftot, tg, packed);
-        if (NW > 1) {
-            lds_r.put(buf, w, lane, rtot);
-            lds_f.put(buf, w, lane, ftot);
-            __syncthreads();
-        }
-        if (CHAIN) {
-            if (w == 0) {
-                NfAgg<VEC> own = lds_r.get(buf, NW - 1, cg);
-#pragma unroll
-                for (int v = NW - 2; v >= 0; --v) { NfAgg<VEC> n = lds_r.get(buf, v, cg); n.after(own); own = n; }
-                nf_chain<VEC, CG>(a, it, pl.b * a.nblk + pl.blk, a.B * a.nblk, cg, tg, own, packed, u);
-                if (tg == 0)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) s_c[cg * VEC + k] = u[k];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) u[k] = s_c[cg * VEC + k];
-        }
+        nf_wave_scan<CG, 1>(rv, rtot, tg);
+        nf_wave_scan<CG, 0>(fw, ftot, tg);
         float su[VEC];
+        if constexpr (CHAIN) {
+            lds_r.put(w, lane, rtot);
+            lds_f.put(w, lane, ftot);
+            __syncthreads();
+            Agg own;
+            if (w == 0) {
+                own = lds_r.get(NW - 1, cg);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) su[k] = u[k];
-        if (NW > 1) {
-#pragma unroll
-            for (int v = NW - 1; v >= 0; --v) {
-                if (v == w)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) su[k] = u[k];
-                lds_r.get(buf, v, cg).apply(u);
+                for (int v = NW - 2; v >= 0; --v) { Agg n = lds_r.get(v, cg); n.after(own); own = n; }
             }
+            if (w < 2) nf_chain_collect<VEC, N, CG, PACKED>(a, w, it, pl.chain, cg, tg, own, s_chain);
+            __syncthreads();
+            nf_chain_enter<VEC, N, CG, PACKED>(a, it, pl.chain, cg, w == 0 && tg == 0, own, s_chain, u);
 #pragma unroll
             for (int v = 0; v < NW - 1; ++v)
-                if (v < w) lds_f.get(buf, v, cg).apply(c);
-        } else rtot.apply(u);
+                if (v < w) lds_f.get(v, cg).apply(c);
+#pragma unroll
+            for (int v = NW - 1; v > 0; --v)
+                if (v > w) lds_r.get(v, cg).apply(u);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) su[k] = u[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) su[k] = u[k];
+            rtot.apply(u);
+        }
         fw.apply(c);
         rv.apply(su);
         // the states in front of every step, then the gradients from the last step to the first
         float hb[TPT][VEC];
 #pragma unroll
         for (int i = 0; i < TPT; ++i) {
-            if (packed && (m.start >> i & 1u)) {
-                const int s = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
+            if (PACKED && (m.start >> i & 1u)) of_sequence(a.h0, j0 + i, c);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) c[k] = a.h0 ? a.h0[(long long)s * a.D + chl + k] : 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) { hb[i][k] = c[k]; c[k] = fmaf(A[i][k], c[k], x[i][k]); }
+            for (int k = 0; k < VEC; ++k) { hb[i][k] = c[k]; c[k] = fmaf(A[i][N == 1 ? 0 : k], c[k], x.at(i, k)); }
         }
         const long long orow = (long long)b * T + row0;
+        char* xq = (char*)a.dx + orow * hstep;
+        char* gq = (char*)a.dgate + orow * gstep;
+        unsigned xo = rows.at(jl + TPT - 1) * (unsigned)hstep + xoff, go = rows.at(jl + TPT - 1) * (unsigned)gstep + goff;
         float dsum[TPT];
 #pragma unroll
         for (int i = TPT - 1; i >= 0; --i) {
             float dx[VEC], dg[VEC];
+            if (PACKED && (m.end >> i & 1u)) of_sequence(a.g_last, j0 + i, su);
             dsum[i] = 0.f;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                dx[k] = ((packed && (m.end >> i & 1u)) ? 0.f : su[k]) + y[i][k];
-                su[k] = A[i][k] * dx[k];
+                dx[k] = su[k] + y.at(i, k);
+                su[k] = A[i][N == 1 ? 0 : k] * dx[k];
                 dg[k] = (a.log_gate ? su[k] : dx[k]) * hb[i][k];
             }
-            if (m.none >> i & 1u)
+            if (PACKED && (m.none >> i & 1u))
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) dx[k] = dg[k] = 0.f;
-            if (live && j0 + i < T) {
+            if (live && (!(PACKED || edge) || j0 + i < T)) {
+                if (SHARED)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) dsum[i] += dg[k];
-                if (a.dx) nf_put<E, VEC>((char*)a.dx + orow * hstep + (unsigned)(rows.at(jl + i) * (unsigned)hstep + xoff), dx);
-                if (!a.shared && a.dgate) {
-                    char* q = (char*)a.dgate + orow * gstep + (unsigned)(rows.at(jl + i) * (unsigned)gstep + goff);
-                    if (ES == 4 || a.gate32) nf_put<NfF32, VEC>(q, dg);
-                    else nf_put<E, VEC>(q, dg);
+                    for (int k = 0; k < VEC; ++k) dsum[i] += dg[k];
+                if (a.dx) nf_put<E, VEC>(xq + xo, dx);
+                if (!SHARED && a.dgate) {
+                    if (ES == 4 || a.gate32) nf_put<NfF32, VEC>(gq + go, dg);
+                    else nf_put<E, VEC>(gq + go, dg);
                 }
-                if (packed && (m.start >> i & 1u) && a.dh0) {
-                    const int q_ = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
+                if (PACKED && (m.start >> i & 1u) && a.dh0) {
+                    const int q = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) a.dh0[(long long)q_ * a.D + ch + k] = su[k];
+                    for (int k = 0; k < VEC; ++k) a.dh0[(long long)q * a.D + ch + k] = su[k];
                 }
             }
+            xo -= rev ? -hstep : hstep;
+            go -= rev ? -gstep : gstep;
         }
-        if (a.shared && a.dgate) {
+        if (SHARED && a.dgate) {
             // sum over the channels of the block: halves of the steps change sides at every level, so that a lane ends with the sums of
             // TPT / CG steps (or a share of one) after TPT - 1 shuffles and a few
             int first = 0;
@@ -694,10 +756,10 @@ __global__ void __launch_bounds__(NW == 1 ? NF_SCAN_WG : 64 * NW) k_scan_bwd(NfS
                     first += up ? n : 0;
                 } else dsum[0] += __shfl_xor(dsum[0], mm);
             }
-            constexpr int N = CG >= TPT ? 1 : TPT / CG, REST = CG >= TPT ? CG / TPT : 1;
+            constexpr int NS = CG >= TPT ? 1 : TPT / CG, REST = CG >= TPT ? CG / TPT : 1;
             if (cg % REST == 0) {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+                for (int i = 0; i < NS; ++i)
                     if (j0 + first + i < T) {
                         const long long o = orow + rows.at(jl + first + i);
                         if (a.nblk > 1) a.dgate_part[(long long)pl.blk * a.B * T + o] = dsum[i];
@@ -706,32 +768,40 @@ __global__ void __launch_bounds__(NW == 1 ? NF_SCAN_WG : 64 * NW) k_scan_bwd(NfS
                     }
             }
         }
-        if (!packed && it == a.ntiles - 1 && a.dh0 && w == 0 && tg == 0 && live)
+        // the tile's first stretch ends with dh0
+        if (!PACKED && it == a.ntiles - 1 && a.dh0 && w == 0 && tg == 0 && live)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) a.dh0[(long long)b * a.D + ch + k] = u[k];
+            for (int k = 0; k < VEC; ++k) a.dh0[(long long)b * a.D + ch + k] = su[k];
     }
 }
 
-// (VEC, CG) -> steps a thread; nw: 1, 4 (whole chains) or -NF_SCAN_CW (a tile a workgroup, chained)
-#define NF_SCAN_CW 4
+// Steps a thread and waves a tile.  A wave on its own (whole chains): NF_SCAN_TPT steps a thread.  Chained tiles, the same steps either way: twice
+// as many on half the waves in the forward, which has the registers for it.
 #define NF_SCAN_TPT(vec) ((vec) == 4 ? 4 : 8)
-template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, int nw, int backward, hipStream_t st)
+#define NF_SCAN_CW 8
+template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st)
 {
     const long long chains = (long long)a.B * a.nblk;
-#define NF_SCAN_GO(V, C, W, CH, GRID)                                                                                                            \
-    if (vec == V && cg == C && nw == (CH ? -W : W)) {                                                                                           \
-        if (backward) hipLaunchKernelGGL((k_scan_bwd<E, V, C, NF_SCAN_TPT(V), W, CH>), dim3((unsigned)(GRID)), dim3(W == 1 ? NF_SCAN_WG : 64 * W), 0, st, a); \
-        else hipLaunchKernelGGL((k_scan_fwd<E, V, C, NF_SCAN_TPT(V), W, CH>), dim3((unsigned)(GRID)), dim3(W == 1 ? NF_SCAN_WG : 64 * W), 0, st, a);          \
-        return 1;                                                                                                                               \
+    const dim3 gw((unsigned)((chains + NF_SCAN_WG / 64 - 1) / (NF_SCAN_WG / 64))), gc((unsigned)(chains * a.ntiles));
+    const int packed = a.sid != nullptr;
+#define NF_SCAN_GO(V, C, CH, PK, SH)                                                                                                              \
+    if (vec == V && cg == C && chain == CH && packed == PK && a.shared == SH) {                                                                  \
+        if (backward) hipLaunchKernelGGL((k_scan_bwd<E, V, C, NF_SCAN_TPT(V), CH ? NF_SCAN_CW : 1, CH, PK, SH>), CH ? gc : gw,                     \
+                                         dim3(CH ? 64 * NF_SCAN_CW : NF_SCAN_WG), 0, st, a);                                                      \
+        else hipLaunchKernelGGL((k_scan_fwd<E, V, C, (CH ? 2 : 1) * NF_SCAN_TPT(V), CH ? NF_SCAN_CW / 2 : 1, CH, PK, SH>), CH ? gc : gw,           \
+                                dim3(CH ? 32 * NF_SCAN_CW : NF_SCAN_WG), 0, st, a);                                                               \
+        return 1;                                                                                                                                \
     }
-#define NF_SCAN_GO_W(V, C) NF_SCAN_GO(V, C, 1, false, (chains + 3) / 4) NF_SCAN_GO(V, C, 4, false, chains) NF_SCAN_GO(V, C, NF_SCAN_CW, true, chains * a.ntiles)
-    NF_SCAN_GO_W(4, 16) NF_SCAN_GO_W(4, 8) NF_SCAN_GO_W(4, 4) NF_SCAN_GO_W(4, 1)
-    NF_SCAN_GO_W(2, 32) NF_SCAN_GO_W(2, 8) NF_SCAN_GO_W(2, 2)
-    NF_SCAN_GO_W(1, 32) NF_SCAN_GO_W(1, 8) NF_SCAN_GO_W(1, 2)
-#undef NF_SCAN_GO_W
+#define NF_SCAN_GO_S(V, C, SH) NF_SCAN_GO(V, C, false, false, SH) NF_SCAN_GO(V, C, true, false, SH) NF_SCAN_GO(V, C, true, true, SH)
+#define NF_SCAN_GO_C(V, C) NF_SCAN_GO_S(V, C, false) NF_SCAN_GO_S(V, C, true)
+    NF_SCAN_GO_C(4, 16) NF_SCAN_GO_C(4, 8) NF_SCAN_GO_C(4, 4) NF_SCAN_GO_C(4, 1)
+    NF_SCAN_GO_C(2, 32) NF_SCAN_GO_C(2, 8) NF_SCAN_GO_C(2, 2)
+    NF_SCAN_GO_C(1, 32) NF_SCAN_GO_C(1, 8) NF_SCAN_GO_C(1, 2)
+#undef NF_SCAN_GO_C
+#undef NF_SCAN_GO_S
 #undef NF_SCAN_GO
     return 0;
 }
-int nf_scan_launch_f32(const NfScanArgs& a, int vec, int cg, int nw, int backward, hipStream_t st);
-int nf_scan_launch_bf16(const NfScanArgs& a, int vec, int cg, int nw, int backward, hipStream_t st);
-int nf_scan_launch_f16(const NfScanArgs& a, int vec, int cg, int nw, int backward, hipStream_t st);
+int nf_scan_launch_f32(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);
+int nf_scan_launch_bf16(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);
+int nf_scan_launch_f16(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);

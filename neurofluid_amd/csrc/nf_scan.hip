@@ -2,8 +2,7 @@
 #include "nf_scan.h"
 #include <math.h>
 
-static int scan_waves(const nf_scan_t* s) { return s->nw < 0 ? -s->nw : s->nw; }
-static int scan_tile(const nf_scan_t* s) { return scan_waves(s) * (64 / s->cg) * NF_SCAN_TPT(s->vec); }
+static int scan_tile(const nf_scan_t* s) { return (s->chain ? NF_SCAN_CW : 1) * (64 / s->cg) * NF_SCAN_TPT(s->vec); }
 static long long scan_blocks(const nf_scan_t* s) { return (s->D + s->cg * s->vec - 1) / (s->cg * s->vec); }
 
 static int scan_check(const nf_scan_t* s, const char* who)
@@ -18,7 +17,7 @@ static int scan_check(const nf_scan_t* s, const char* who)
 static bool scan_plan_ok(const nf_scan_t* s)
 {
     const bool lanes = s->vec == 4 ? (s->cg == 16 || s->cg == 8 || s->cg == 4 || s->cg == 1) : ((s->vec == 2 || s->vec == 1) && (s->cg == 32 || s->cg == 8 || s->cg == 2));
-    return lanes && (s->nw == 1 || s->nw == 4 || s->nw == -NF_SCAN_CW) && s->D % s->vec == 0;
+    return lanes && (s->chain == 0 || s->chain == 1) && (s->chain || !s->row_splits) && s->D % s->vec == 0;
 }
 
 // elements that every row which (base, strides) reaches can be read at a time: 4, 2 or 1
@@ -29,8 +28,8 @@ static int scan_vec(const void* p, int64_t sb, int64_t st, int size)
     return v;
 }
 
-// Lanes: as many channels a block as D has, 64 at the most.  Waves: a chain of few steps, or one of thousands, keeps to a wave (no
-// barrier); below 1 024 chains the tiles of a chain go to workgroups of their own.
+// Lanes: as many channels a block as D has, 64 at the most.  Waves: thousands of chains, or chains of few steps, take a wave each; else the
+// tiles of a chain go to workgroups of their own.
 extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
 {
     const int rc = scan_check(s, __func__);
@@ -43,28 +42,29 @@ extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
     if (v == 4) s->cg = s->D <= 4 ? 1 : s->D <= 16 ? 4 : s->D <= 32 ? 8 : 16;
     else s->cg = s->D <= 2 * v ? 2 : s->D <= 8 * v ? 8 : 32;
     const long long chains = (long long)s->B * scan_blocks(s);
-    s->nw = 1;
-    const int t1 = scan_tile(s);
-    if (s->T > t1 && (s->row_splits || (chains < 4096 && s->T > 2 * t1))) {
-        s->nw = 4;
-        if (s->T > scan_tile(s) && chains < 1024) s->nw = -NF_SCAN_CW;
-    }
+    s->chain = 0;
+    s->chain = s->row_splits || (chains < 4096 && s->T > 2 * scan_tile(s));
     const int tile = scan_tile(s);
     if (state_floats) *state_floats = (size_t)s->B * ((s->T + tile - 1) / tile) * s->D;
     return NF_OK;
 }
 
-// workspace, in 8-byte words: [tile | group | set entries | ticket] of the chained kernels, then the per-block sums of a shared gate's gradient
-struct ScanWs { size_t tile, group, set, part; size_t entries() const { return tile + group + set; } size_t words() const { return (entries() ? entries() + 1 : 0) + (part + 1) / 2; } };
+// workspace, in 8-byte words: [tile | group | set entries | counters] of the chained kernels, then the per-block sums of a shared gate's gradient
+struct ScanWs {
+    size_t tile, group, set, counters, part;
+    size_t entries() const { return tile + group + set; }
+    size_t words() const { return entries() + counters + (part + 1) / 2; }
+};
 static ScanWs scan_workspace(const nf_scan_t* s, int backward)
 {
-    ScanWs w = {0, 0, 0, 0};
-    if (s->nw < 0) {
+    ScanWs w = {0, 0, 0, 0, 0};
+    if (s->chain) {
         const int tile = scan_tile(s);
         const size_t per = (size_t)s->B * scan_blocks(s) * s->cg * s->vec, nt = (s->T + tile - 1) / tile;
         w.tile = nt * per;
         w.group = (nt + NF_SCAN_FAN - 1) / NF_SCAN_FAN * per;
         w.set = (nt + NF_SCAN_FAN * NF_SCAN_FAN - 1) / (NF_SCAN_FAN * NF_SCAN_FAN) * per;
+        w.counters = (size_t)s->B * scan_blocks(s) * NF_SCAN_LINE / 2;
     }
     if (backward && s->shared && s->dgate && scan_blocks(s) > 1) w.part = (size_t)scan_blocks(s) * s->B * s->T;
     return w;
@@ -102,10 +102,10 @@ __global__ void __launch_bounds__(256) k_scan_empty(const int64_t* __restrict__ 
     if (a >= b) dst[e] = src ? src[e] : 0.f;
 }
 
-// The chain's entries are set to "empty", the counter of tiles to 0 (a kernel: a memset node in a captured graph has given wrong results).
-__global__ void __launch_bounds__(256) k_scan_clear(unsigned long long* __restrict__ w, size_t entries)
+// The chain's entries are set to "empty", the counters of tiles to 0 (a kernel: a memset node in a captured graph has given wrong results).
+__global__ void __launch_bounds__(256) k_scan_clear(unsigned long long* __restrict__ w, size_t entries, size_t n)
 {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i <= entries; i += (size_t)gridDim.x * 256) w[i] = i < entries ? NF_SCAN_EMPTY : 0ull;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) w[i] = i < entries ? NF_SCAN_EMPTY : 0ull;
 }
 
 __global__ void __launch_bounds__(256) k_scan_fold(const float* __restrict__ part, int nblk, long long n, int type, void* __restrict__ out)
@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(256) k_scan_fold(const float* __restrict__ par
 
 static int scan_go(const nf_scan_t* s, const NfScanArgs& a, int backward, hipStream_t st)
 {
-    if (s->dtype == 0) return nf_scan_launch_f32(a, s->vec, s->cg, s->nw, backward, st);
-    if (s->dtype == 1) return nf_scan_launch_bf16(a, s->vec, s->cg, s->nw, backward, st);
-    return nf_scan_launch_f16(a, s->vec, s->cg, s->nw, backward, st);
+    if (s->dtype == 0) return nf_scan_launch_f32(a, s->vec, s->cg, s->chain, backward, st);
+    if (s->dtype == 1) return nf_scan_launch_bf16(a, s->vec, s->cg, s->chain, backward, st);
+    return nf_scan_launch_f16(a, s->vec, s->cg, s->chain, backward, st);
 }
 
 static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char* who)
@@ -167,7 +167,7 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     a.nblk = (int)scan_blocks(s);
     a.ntiles = (s->T + tile - 1) / tile;
     a.gate32 = s->gate32 != 0; a.shared = s->shared != 0; a.log_gate = s->log_gate != 0; a.reverse = s->reverse != 0;
-    if ((long long)a.B * a.nblk * (s->nw < 0 ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
+    if ((long long)a.B * a.nblk * (s->chain ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
     const ScanWs ws = scan_workspace(s, backward);
     const size_t n_part = ws.part;
     if (s->workspace_bytes < 8 * ws.words() || (ws.words() && (!s->workspace || (uintptr_t)s->workspace % 8))) {
@@ -176,14 +176,14 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     }
     unsigned long long* words = (unsigned long long*)s->workspace;
     a.ws_tile = words; a.ws_group = words + ws.tile; a.ws_set = a.ws_group + ws.group; a.ticket = (int*)(words + ws.entries());
-    a.dgate_part = n_part ? (float*)(words + (ws.entries() ? ws.entries() + 1 : 0)) : nullptr;
+    a.dgate_part = n_part ? (float*)(words + ws.entries() + ws.counters) : nullptr;
     if (packed && !backward) {
         hipLaunchKernelGGL(k_scan_rows, dim3((unsigned)((s->T + 255) / 256)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->sid);
         NF_CHECK_LAUNCH();
     }
     if (ws.entries()) {
-        const size_t blocks = (ws.entries() + 256) / 256;
-        hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, words, ws.entries());
+        const size_t n = ws.entries() + ws.counters, blocks = (n + 255) / 256;
+        hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, words, ws.entries(), n);
         NF_CHECK_LAUNCH();
     }
     if (!scan_go(s, a, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
