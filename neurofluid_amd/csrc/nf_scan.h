@@ -329,7 +329,18 @@ template <int VEC, int N, bool PACKED> struct NfEntry {
     }
     __device__ __forceinline__ NfAgg<VEC, N, PACKED> wait(const unsigned long long* p)
     {
-        while (missing()) { __builtin_amdgcn_s_sleep(2); ask(p); }      // (a pause: the polls go past the caches)
+        // Polls go past the caches to memory that every XCD shares, so one lane polls one word for all that wait, and they read again
+        // when it is there (an entry's words are stored together: most often once).
+        for (unsigned long long m = __ballot(missing()); m != 0; m = __ballot(missing())) {
+            if ((int)(threadIdx.x & 63) == __ffsll((long long)m) - 1) {
+                int k = 0;
+#pragma unroll
+                for (int i = VEC - 1; i > 0; --i)
+                    if (w[i] == NF_SCAN_EMPTY) k = i;
+                while (__hip_atomic_load(p + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == NF_SCAN_EMPTY) __builtin_amdgcn_s_sleep(1);
+            }
+            if (missing()) ask(p);
+        }
         NfAgg<VEC, N, PACKED> t;
         t.closed = 0;
 #pragma unroll
