@@ -590,7 +590,7 @@ int nf_trans_step(const nf_trans_step_t* s /*[host]*/, const float* pos, const f
  * with u behind the last step = g_last.  States, products and sums are fp32; what is stored in 16 bits is rounded once, to nearest.
  * The stretch products carry states over long distances: gates are meant to be decays (|A| <= 1), larger ones overflow there sooner than
  * step by step.  Results repeat bit for bit.
- * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, chain; *state_floats = the size
+ * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, mode; *state_floats = the size
  * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_bytes =
  * nf_scan_workspace_bytes(s, backward) bytes, 8-byte aligned, for this call alone.  T <= 2^30, D <= 2^20, step strides < 2^19 elements or so (a tile's rows span less than 2^31 bytes).  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
  * h0, states (and sid).
@@ -606,7 +606,7 @@ typedef struct {
     int64_t gate_sb, gate_st, x_sb, x_st, g_sb, g_st;
     void* h; float* h_last; float* states /*forward: or NULL*/; int32_t* sid /*packed*/;
     void* dgate /*or NULL*/; void* dx /*or NULL*/; float* dh0 /*or NULL*/;
-    int vec, cg, chain;
+    int vec, cg, mode;
     void* workspace; size_t workspace_bytes;
 } nf_scan_t;
 int nf_scan_plan(nf_scan_t* s /*[host]*/, size_t* state_floats /*[host]*/);

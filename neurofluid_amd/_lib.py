@@ -32,7 +32,7 @@ class Scan(ctypes.Structure):
                [(k, c_void_p) for k in ("row_splits", "gate", "x", "g", "h0", "g_last")] + \
                [(k, c_int64) for k in ("gate_sb", "gate_st", "x_sb", "x_st", "g_sb", "g_st")] + \
                [(k, c_void_p) for k in ("h", "h_last", "states", "sid", "dgate", "dx", "dh0")] + \
-               [(k, c_int) for k in ("vec", "cg", "chain")] + [("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+               [(k, c_int) for k in ("vec", "cg", "mode")] + [("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
 class Act8Job(ctypes.Structure):

@@ -15,8 +15,9 @@
 // Lanes: CG channel groups of VEC adjacent channels x 64 / CG stretches; NW waves share a tile.
 //
 // A (sequence, block of channels) is a chain; its tiles follow one another.
-//   many chains (CHAIN = false): a wave walks a whole chain, four independent ones a workgroup, no barrier;
-//   few chains (CHAIN = true): a workgroup takes ONE tile.  It publishes the tile's (P, H), collects those of the tiles in front of it and goes on
+//   very many, or short ones (NF_SCAN_WAVE): a wave walks a whole chain, four independent ones a workgroup, no barrier;
+//   many (NF_SCAN_WALK): a workgroup walks a whole chain;
+//   few (NF_SCAN_CHAIN): a workgroup takes ONE tile.  It publishes the tile's (P, H), collects those of the tiles in front of it and goes on
 //     with the state they make: every tensor is still read and written once.  The collection has a fixed shape, whatever the order of
 //     arrival: tiles in groups of 16, groups in sets of 16; a group's last tile publishes the group's (P, H), a set's last tile the state behind it;
 //     a tile composes the set's state, the groups of its set and the tiles of its group in front of it, at most 31 entries.
@@ -26,6 +27,9 @@
 #pragma once
 #include "nf_common.h"
 
+#define NF_SCAN_WAVE 0
+#define NF_SCAN_CHAIN 1
+#define NF_SCAN_WALK 2
 #define NF_SCAN_WG 256
 #define NF_SCAN_MAX_STEPS (1 << 30)
 #define NF_SCAN_MAX_CHANNELS (1 << 20)
@@ -421,19 +425,23 @@ __device__ __forceinline__ void nf_chain_enter(const NfScanArgs& a, int k, int c
     }
 }
 
-// A wave's place: its chain, and for CHAIN the workgroup's tile by ticket.
+// A wave's place: its chain, and for NF_SCAN_CHAIN the workgroup's tile by ticket.
 struct NfPlace { int blk, b, k, w, chain; bool ok; };
-template <bool CHAIN> __device__ __forceinline__ NfPlace nf_place(const NfScanArgs& a)
+template <int MODE> __device__ __forceinline__ NfPlace nf_place(const NfScanArgs& a)
 {
     __shared__ int s_ticket;
     NfPlace p;
     const int nchains = a.B * a.nblk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (CHAIN) {
+    if (MODE == NF_SCAN_CHAIN) {
         p.chain = blockIdx.x % nchains;
         if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(a.ticket + p.chain * NF_SCAN_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         p.k = __builtin_amdgcn_readfirstlane(s_ticket);
+        p.w = wave;
+    } else if (MODE == NF_SCAN_WALK) {
+        p.chain = blockIdx.x;
+        p.k = 0;
         p.w = wave;
     } else {
         p.chain = blockIdx.x * (NF_SCAN_WG / 64) + wave;
@@ -451,14 +459,15 @@ template <int TPT> __device__ __forceinline__ unsigned nf_beyond(int j0, int T) 
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN, bool PACKED, bool SHARED>
-__global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_fwd(NfScanArgs a)
+template <typename E, int VEC, int CG, int TPT, int NW, int MODE, bool PACKED, bool SHARED>
+__global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k_scan_fwd(NfScanArgs a)
 {
     constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st), N = SHARED ? 1 : VEC;
     typedef NfAgg<VEC, N, PACKED> Agg;
-    __shared__ NfScanLds<VEC, N, CG, CHAIN ? NW : 1, PACKED> lds;
+    constexpr bool CHAIN = MODE == NF_SCAN_CHAIN, WAVE = MODE == NF_SCAN_WAVE;
+    __shared__ NfScanLds<VEC, N, CG, NW, PACKED> lds_[CHAIN ? 1 : 2];     // two for a walk: one barrier a tile is enough, a wave is at most one tile ahead
     __shared__ NfChainLds<VEC, N, CG, PACKED> s_chain;
-    const NfPlace pl = nf_place<CHAIN>(a);
+    const NfPlace pl = nf_place<MODE>(a);
     if (!pl.ok) return;                                  // (whole chains by waves only: no barrier below)
     const int lane = threadIdx.x & 63, cg = lane % CG, tg = lane / CG, w = pl.w, b = pl.b;
     const int ch = (pl.blk * CG + cg) * VEC;
@@ -525,9 +534,12 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_fwd(NfSca
         }
         nf_wave_scan<CG, 0>(me, tot, tg);
         float s[VEC];
-        if constexpr (CHAIN) {
+        auto& lds = lds_[CHAIN ? 0 : tile & 1];
+        if constexpr (!WAVE) {
             lds.put(w, lane, tot);
             __syncthreads();
+        }
+        if constexpr (CHAIN) {
             Agg own;
             if (w == 0) {
                 own = lds.get(0, cg);
@@ -541,12 +553,14 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_fwd(NfSca
         if (a.states && w == 0 && tg == 0 && live)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) a.states[((long long)b * a.ntiles + tile) * a.D + ch + k] = c[k];
-        if constexpr (CHAIN) {
+        if constexpr (!WAVE) {
 #pragma unroll
-            for (int v = 0; v < NW - 1; ++v)
-                if (v < w) lds.get(v, cg).apply(c);
+            for (int v = 0; v < NW; ++v) {
+                if (v == w)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) s[k] = c[k];
+                    for (int k = 0; k < VEC; ++k) s[k] = c[k];
+                if (!CHAIN || v < w) lds.get(v, cg).apply(c);
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) s[k] = c[k];
@@ -590,14 +604,15 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_fwd(NfSca
 // ------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------
-template <typename E, int VEC, int CG, int TPT, int NW, bool CHAIN, bool PACKED, bool SHARED>
-__global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_bwd(NfScanArgs a)
+template <typename E, int VEC, int CG, int TPT, int NW, int MODE, bool PACKED, bool SHARED>
+__global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k_scan_bwd(NfScanArgs a)
 {
     constexpr int TG = 64 / CG, TS = NW * TG * TPT, ES = sizeof(typename E::st), N = SHARED ? 1 : VEC;
     typedef NfAgg<VEC, N, PACKED> Agg;
-    __shared__ NfScanLds<VEC, N, CG, CHAIN ? NW : 1, PACKED> lds_f, lds_r;
+    constexpr bool CHAIN = MODE == NF_SCAN_CHAIN, WAVE = MODE == NF_SCAN_WAVE;
+    __shared__ NfScanLds<VEC, N, CG, NW, PACKED> lds_f_[CHAIN ? 1 : 2], lds_r_[CHAIN ? 1 : 2];
     __shared__ NfChainLds<VEC, N, CG, PACKED> s_chain;
-    const NfPlace pl = nf_place<CHAIN>(a);
+    const NfPlace pl = nf_place<MODE>(a);
     if (!pl.ok) return;
     const int lane = threadIdx.x & 63, cg = lane % CG, tg = lane / CG, w = pl.w, b = pl.b;
     const int ch = (pl.blk * CG + cg) * VEC;
@@ -676,10 +691,14 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_bwd(NfSca
         nf_wave_scan<CG, 1>(rv, rtot, tg);
         nf_wave_scan<CG, 0>(fw, ftot, tg);
         float su[VEC];
-        if constexpr (CHAIN) {
+        auto& lds_r = lds_r_[CHAIN ? 0 : it & 1];
+        auto& lds_f = lds_f_[CHAIN ? 0 : it & 1];
+        if constexpr (!WAVE) {
             lds_r.put(w, lane, rtot);
             lds_f.put(w, lane, ftot);
             __syncthreads();
+        }
+        if constexpr (CHAIN) {
             Agg own;
             if (w == 0) {
                 own = lds_r.get(NW - 1, cg);
@@ -689,14 +708,18 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_bwd(NfSca
             if (w < 2) nf_chain_collect<VEC, N, CG, PACKED>(a, w, it, pl.chain, cg, tg, own, s_chain);
             __syncthreads();
             nf_chain_enter<VEC, N, CG, PACKED>(a, it, pl.chain, cg, w == 0 && tg == 0, own, s_chain, u);
+        }
+        if constexpr (!WAVE) {
 #pragma unroll
             for (int v = 0; v < NW - 1; ++v)
                 if (v < w) lds_f.get(v, cg).apply(c);
 #pragma unroll
-            for (int v = NW - 1; v > 0; --v)
-                if (v > w) lds_r.get(v, cg).apply(u);
+            for (int v = NW - 1; v >= 0; --v) {
+                if (v == w)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) su[k] = u[k];
+                    for (int k = 0; k < VEC; ++k) su[k] = u[k];
+                if (!CHAIN || v > w) lds_r.get(v, cg).apply(u);
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) su[k] = u[k];
@@ -786,24 +809,26 @@ __global__ void __launch_bounds__(CHAIN ? 64 * NW : NF_SCAN_WG) k_scan_bwd(NfSca
     }
 }
 
-// Steps a thread and waves a tile.  A wave on its own (whole chains): NF_SCAN_TPT steps a thread.  Chained tiles, the same steps either way: twice
-// as many on half the waves in the forward, which has the registers for it.
-#define NF_SCAN_TPT(vec) ((vec) == 4 ? 4 : 8)
-#define NF_SCAN_CW 8
-template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st)
+// Steps a thread and waves a tile.  A wave on its own: NF_SCAN_TPT steps a thread; else twice as many (half the exchange for a step) on NF_SCAN_NW waves.
+#define NF_SCAN_TPT(vec, mode) (((vec) == 4 ? 4 : 8) * ((mode) == NF_SCAN_WAVE ? 1 : 2))
+#ifndef NF_SCAN_NWC
+#define NF_SCAN_NWC 8
+#define NF_SCAN_NWW 8
+#endif
+#define NF_SCAN_NW(mode) ((mode) == NF_SCAN_WAVE ? 1 : (mode) == NF_SCAN_CHAIN ? NF_SCAN_NWC : NF_SCAN_NWW)
+template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, int mode, int backward, hipStream_t st)
 {
     const long long chains = (long long)a.B * a.nblk;
-    const dim3 gw((unsigned)((chains + NF_SCAN_WG / 64 - 1) / (NF_SCAN_WG / 64))), gc((unsigned)(chains * a.ntiles));
+    const dim3 grid((unsigned)(mode == NF_SCAN_WAVE ? (chains + NF_SCAN_WG / 64 - 1) / (NF_SCAN_WG / 64) : mode == NF_SCAN_WALK ? chains : chains * a.ntiles));
     const int packed = a.sid != nullptr;
-#define NF_SCAN_GO(V, C, CH, PK, SH)                                                                                                              \
-    if (vec == V && cg == C && chain == CH && packed == PK && a.shared == SH) {                                                                  \
-        if (backward) hipLaunchKernelGGL((k_scan_bwd<E, V, C, NF_SCAN_TPT(V), CH ? NF_SCAN_CW : 1, CH, PK, SH>), CH ? gc : gw,                     \
-                                         dim3(CH ? 64 * NF_SCAN_CW : NF_SCAN_WG), 0, st, a);                                                      \
-        else hipLaunchKernelGGL((k_scan_fwd<E, V, C, (CH ? 2 : 1) * NF_SCAN_TPT(V), CH ? NF_SCAN_CW / 2 : 1, CH, PK, SH>), CH ? gc : gw,           \
-                                dim3(CH ? 32 * NF_SCAN_CW : NF_SCAN_WG), 0, st, a);                                                               \
-        return 1;                                                                                                                                \
+#define NF_SCAN_GO(V, C, M, PK, SH)                                                                                                                          \
+    if (vec == V && cg == C && mode == M && packed == PK && a.shared == SH) {                                                                               \
+        constexpr int NW = NF_SCAN_NW(M), TH = M == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW, TPT = NF_SCAN_TPT(V, M);                                             \
+        if (backward) hipLaunchKernelGGL((k_scan_bwd<E, V, C, TPT, NW, M, PK, SH>), grid, dim3(TH), 0, st, a);                                               \
+        else hipLaunchKernelGGL((k_scan_fwd<E, V, C, TPT, NW, M, PK, SH>), grid, dim3(TH), 0, st, a);                                                        \
+        return 1;                                                                                                                                           \
     }
-#define NF_SCAN_GO_S(V, C, SH) NF_SCAN_GO(V, C, false, false, SH) NF_SCAN_GO(V, C, true, false, SH) NF_SCAN_GO(V, C, true, true, SH)
+#define NF_SCAN_GO_S(V, C, SH) NF_SCAN_GO(V, C, NF_SCAN_WAVE, false, SH) NF_SCAN_GO(V, C, NF_SCAN_WALK, false, SH) NF_SCAN_GO(V, C, NF_SCAN_CHAIN, false, SH) NF_SCAN_GO(V, C, NF_SCAN_CHAIN, true, SH)
 #define NF_SCAN_GO_C(V, C) NF_SCAN_GO_S(V, C, false) NF_SCAN_GO_S(V, C, true)
     NF_SCAN_GO_C(4, 16) NF_SCAN_GO_C(4, 8) NF_SCAN_GO_C(4, 4) NF_SCAN_GO_C(4, 1)
     NF_SCAN_GO_C(2, 32) NF_SCAN_GO_C(2, 8) NF_SCAN_GO_C(2, 2)
@@ -813,6 +838,6 @@ template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, i
 #undef NF_SCAN_GO
     return 0;
 }
-int nf_scan_launch_f32(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);
-int nf_scan_launch_bf16(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);
-int nf_scan_launch_f16(const NfScanArgs& a, int vec, int cg, int chain, int backward, hipStream_t st);
+int nf_scan_launch_f32(const NfScanArgs& a, int vec, int cg, int mode, int backward, hipStream_t st);
+int nf_scan_launch_bf16(const NfScanArgs& a, int vec, int cg, int mode, int backward, hipStream_t st);
+int nf_scan_launch_f16(const NfScanArgs& a, int vec, int cg, int mode, int backward, hipStream_t st);

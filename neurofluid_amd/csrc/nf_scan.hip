@@ -1,8 +1,9 @@
 // nf_scan.hip — entry points of the gated linear recurrence (kernels: nf_scan.h).
 #include "nf_scan.h"
 #include <math.h>
+#include <stdlib.h>
 
-static int scan_tile(const nf_scan_t* s) { return (s->chain ? NF_SCAN_CW : 1) * (64 / s->cg) * NF_SCAN_TPT(s->vec); }
+static int scan_tile(const nf_scan_t* s) { return NF_SCAN_NW(s->mode) * (64 / s->cg) * NF_SCAN_TPT(s->vec, s->mode); }
 static long long scan_blocks(const nf_scan_t* s) { return (s->D + s->cg * s->vec - 1) / (s->cg * s->vec); }
 
 static int scan_check(const nf_scan_t* s, const char* who)
@@ -17,7 +18,7 @@ static int scan_check(const nf_scan_t* s, const char* who)
 static bool scan_plan_ok(const nf_scan_t* s)
 {
     const bool lanes = s->vec == 4 ? (s->cg == 16 || s->cg == 8 || s->cg == 4 || s->cg == 1) : ((s->vec == 2 || s->vec == 1) && (s->cg == 32 || s->cg == 8 || s->cg == 2));
-    return lanes && (s->chain == 0 || s->chain == 1) && (s->chain || !s->row_splits) && s->D % s->vec == 0;
+    return lanes && s->mode >= 0 && s->mode <= 2 && (s->mode == NF_SCAN_CHAIN || !s->row_splits) && s->D % s->vec == 0;
 }
 
 // elements that every row which (base, strides) reaches can be read at a time: 4, 2 or 1
@@ -28,6 +29,7 @@ static int scan_vec(const void* p, int64_t sb, int64_t st, int size)
     return v;
 }
 
+static long long scan_walk_min() { const char* e = getenv("NF_WALK_MIN"); return e ? atoi(e) : 128; }
 // Lanes: as many channels a block as D has, 64 at the most.  Waves: thousands of chains, or chains of few steps, take a wave each; else the
 // tiles of a chain go to workgroups of their own.
 extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
@@ -42,8 +44,9 @@ extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
     if (v == 4) s->cg = s->D <= 4 ? 1 : s->D <= 16 ? 4 : s->D <= 32 ? 8 : 16;
     else s->cg = s->D <= 2 * v ? 2 : s->D <= 8 * v ? 8 : 32;
     const long long chains = (long long)s->B * scan_blocks(s);
-    s->chain = 0;
-    s->chain = s->row_splits || (chains < 4096 && s->T > 2 * scan_tile(s));
+    s->mode = NF_SCAN_WAVE;
+    if (s->row_splits) s->mode = NF_SCAN_CHAIN;
+    else if (chains < 4096 && s->T > 2 * scan_tile(s)) s->mode = chains >= scan_walk_min() ? NF_SCAN_WALK : NF_SCAN_CHAIN;
     const int tile = scan_tile(s);
     if (state_floats) *state_floats = (size_t)s->B * ((s->T + tile - 1) / tile) * s->D;
     return NF_OK;
@@ -58,7 +61,7 @@ struct ScanWs {
 static ScanWs scan_workspace(const nf_scan_t* s, int backward)
 {
     ScanWs w = {0, 0, 0, 0, 0};
-    if (s->chain) {
+    if (s->mode == NF_SCAN_CHAIN) {
         const int tile = scan_tile(s);
         const size_t per = (size_t)s->B * scan_blocks(s) * s->cg * s->vec, nt = (s->T + tile - 1) / tile;
         w.tile = nt * per;
@@ -121,9 +124,9 @@ __global__ void __launch_bounds__(256) k_scan_fold(const float* __restrict__ par
 
 static int scan_go(const nf_scan_t* s, const NfScanArgs& a, int backward, hipStream_t st)
 {
-    if (s->dtype == 0) return nf_scan_launch_f32(a, s->vec, s->cg, s->chain, backward, st);
-    if (s->dtype == 1) return nf_scan_launch_bf16(a, s->vec, s->cg, s->chain, backward, st);
-    return nf_scan_launch_f16(a, s->vec, s->cg, s->chain, backward, st);
+    if (s->dtype == 0) return nf_scan_launch_f32(a, s->vec, s->cg, s->mode, backward, st);
+    if (s->dtype == 1) return nf_scan_launch_bf16(a, s->vec, s->cg, s->mode, backward, st);
+    return nf_scan_launch_f16(a, s->vec, s->cg, s->mode, backward, st);
 }
 
 static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char* who)
@@ -167,7 +170,7 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     a.nblk = (int)scan_blocks(s);
     a.ntiles = (s->T + tile - 1) / tile;
     a.gate32 = s->gate32 != 0; a.shared = s->shared != 0; a.log_gate = s->log_gate != 0; a.reverse = s->reverse != 0;
-    if ((long long)a.B * a.nblk * (s->chain ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
+    if ((long long)a.B * a.nblk * (s->mode == NF_SCAN_CHAIN ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
     const ScanWs ws = scan_workspace(s, backward);
     const size_t n_part = ws.part;
     if (s->workspace_bytes < 8 * ws.words() || (ws.words() && (!s->workspace || (uintptr_t)s->workspace % 8))) {

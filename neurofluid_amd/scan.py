@@ -89,7 +89,7 @@ class _ScanFn(torch.autograd.Function):
                 check(lib.nf_scan_fwd(ctypes.byref(s), _lib.stream()), "nf_scan_fwd")
         if need:
             ctx.save_for_backward(gate, x, h0, row_splits, states, sid)
-            ctx.opts, ctx.plan = (log_gate, reverse), (s.vec, s.cg, s.chain)
+            ctx.opts, ctx.plan = (log_gate, reverse), (s.vec, s.cg, s.mode)
         return h, last
 
     @staticmethod
@@ -104,7 +104,7 @@ class _ScanFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         with torch.cuda.device(dev):
             s = _describe(g_, x_, row_splits, *ctx.opts)
-            s.vec, s.cg, s.chain = ctx.plan
+            s.vec, s.cg, s.mode = ctx.plan
             n_state = s.n_seq if row_splits is not None else s.B
             dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[0] else None
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[1] else None
