@@ -1,7 +1,6 @@
 // nf_scan.hip — entry points of the gated linear recurrence (kernels: nf_scan.h).
 #include "nf_scan.h"
 #include <math.h>
-#include <stdlib.h>
 
 static int scan_tile(const nf_scan_t* s) { return NF_SCAN_NW(s->mode) * (64 / s->cg) * NF_SCAN_TPT(s->vec, s->mode); }
 static long long scan_blocks(const nf_scan_t* s) { return (s->D + s->cg * s->vec - 1) / (s->cg * s->vec); }
@@ -29,9 +28,10 @@ static int scan_vec(const void* p, int64_t sb, int64_t st, int size)
     return v;
 }
 
-static long long scan_walk_min() { const char* e = getenv("NF_WALK_MIN"); return e ? atoi(e) : 128; }
-// Lanes: as many channels a block as D has, 64 at the most.  Waves: thousands of chains, or chains of few steps, take a wave each; else the
-// tiles of a chain go to workgroups of their own.
+// Lanes: as many channels a block as D has, a cache line's 64 of 16 bits or 32 of 32 bits at the most (65 536 steps x 256 channels in fp32: 46 us
+// forward with 32, 52 with 64; in fp16 43 with 64, 45 with 32).  Modes: thousands of chains, or chains of few steps, take a wave each; from 8 192 channels on a
+// workgroup each (2048 steps, fp16, forward / backward: 16 384 channels 40 / 76 us against 59 / 92 chained, 8 192 29 / 46 against 31 / 46,
+// 4 096 and 4096 steps 47 / 77 against 33 / 46); fewer ones are chained.
 extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
 {
     const int rc = scan_check(s, __func__);
@@ -41,12 +41,12 @@ extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
     if (!s->shared) { const int vg = scan_vec(s->gate, s->gate_sb, s->gate_st, gs); v = vg < v ? vg : v; }
     while (s->D % v) v /= 2;
     s->vec = v;
-    if (v == 4) s->cg = s->D <= 4 ? 1 : s->D <= 16 ? 4 : s->D <= 32 ? 8 : 16;
+    if (v == 4) s->cg = s->D <= 4 ? 1 : s->D <= 16 ? 4 : s->D <= 32 || s->dtype == 0 ? 8 : 16;
     else s->cg = s->D <= 2 * v ? 2 : s->D <= 8 * v ? 8 : 32;
     const long long chains = (long long)s->B * scan_blocks(s);
     s->mode = NF_SCAN_WAVE;
     if (s->row_splits) s->mode = NF_SCAN_CHAIN;
-    else if (chains < 4096 && s->T > 2 * scan_tile(s)) s->mode = chains >= scan_walk_min() ? NF_SCAN_WALK : NF_SCAN_CHAIN;
+    else if (chains < 4096 && s->T > 2 * scan_tile(s)) s->mode = chains * s->cg * s->vec >= 8192 ? NF_SCAN_WALK : NF_SCAN_CHAIN;
     const int tile = scan_tile(s);
     if (state_floats) *state_floats = (size_t)s->B * ((s->T + tile - 1) / tile) * s->D;
     return NF_OK;
