@@ -231,3 +231,25 @@ def ptr(t):
 def stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(fn):
+    """Decorator for an entry point whose first argument is a tensor: runs it with that tensor's device as the current one (entered only if it is
+    not already: the guard and the stream object of torch.cuda cost as much as a small launch)."""
+    import functools
+    import torch
+
+    @functools.wraps(fn)
+    def call(t, *args, **kw):
+        dev = t.get_device()
+        if dev < 0 or dev == torch.cuda.current_device():
+            return fn(t, *args, **kw)
+        with torch.cuda.device(dev):
+            return fn(t, *args, **kw)
+    return call
+
+
+def raw_stream(t):
+    """The current stream of t's device as the C ABI takes it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(t.get_device())

@@ -54,12 +54,7 @@ class Act8:
         dtype = dtype or self.dtype
         if dtype not in _DTYPES:
             raise TypeError(f"Act8.unpack: float32, bfloat16 or float16, not {dtype}")
-        lib = _lib.load()
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            check(lib.nf_act8_unpack(_DTYPES[dtype], ptr(self.codes), ptr(self.scales), self.rows, self.features, ptr(out), self.features, _lib.stream()),
-                  "nf_act8_unpack")
-        return out
+        return _unpack(self.codes, self, dtype)
 
 
 def pack(x):
@@ -73,14 +68,28 @@ def pack(x):
     if rows > _MAX or x.shape[-1] > _MAX:
         raise ValueError(f"act8.pack: more than {_MAX} rows or features")
     ops._require_cuda(x)
+    return _pack(x, rows)
+
+
+@_lib.on_device
+def _pack(x, rows):
     lib = _lib.load()
-    with torch.cuda.device(x.device):
-        m = _matrix(x.detach()) if rows else x.detach()
-        codes = torch.empty(lib.nf_act8_code_bytes(rows, x.shape[-1]), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(lib.nf_act8_scale_bytes(rows, x.shape[-1]), dtype=torch.uint8, device=x.device)
-        if rows:
-            check(lib.nf_act8_pack(_DTYPES[x.dtype], ptr(m), m.stride(0), rows, x.shape[-1], ptr(codes), ptr(scales), _lib.stream()), "nf_act8_pack")
+    K = x.shape[-1]
+    m = _matrix(x.detach()) if rows else x.detach()
+    n_codes = lib.nf_act8_code_bytes(rows, K)         # (a multiple of 32)
+    both = torch.empty(n_codes + lib.nf_act8_scale_bytes(rows, K), dtype=torch.uint8, device=x.device)
+    codes, scales = both[:n_codes], both[n_codes:]
+    if rows and K:
+        check(lib.nf_act8_pack(_DTYPES[x.dtype], m.data_ptr(), m.stride(0), rows, K, codes.data_ptr(), scales.data_ptr(), _lib.raw_stream(x)), "nf_act8_pack")
     return Act8(codes, scales, x.shape, x.dtype)
+
+
+@_lib.on_device
+def _unpack(codes, ck, dtype):
+    out = torch.empty(ck.shape, dtype=dtype, device=codes.device)
+    check(_lib.load().nf_act8_unpack(_DTYPES[dtype], codes.data_ptr(), ck.scales.data_ptr(), ck.rows, ck.features, out.data_ptr(), ck.features,
+                                     _lib.raw_stream(codes)), "nf_act8_unpack")
+    return out
 
 
 def wgrad_jobs(dy, ckpt, jobs):
@@ -97,18 +106,22 @@ def wgrad_jobs(dy, ckpt, jobs):
     ops._require_cuda(dy)
     if dy.device != ckpt.device:
         raise ValueError("act8.wgrad: dy and the activations are on different devices")
+    return _wgrad(dy, ckpt, jobs)
+
+
+@_lib.on_device
+def _wgrad(dy, ckpt, jobs):
     lib = _lib.load()
-    dev = dy.device
-    with torch.cuda.device(dev):
-        m = _matrix(dy.detach())
-        js = (_lib.Act8Job * len(jobs))(*[_lib.Act8Job(int(a), int(b), int(c), int(d), int(bool(e))) for a, b, c, d, e in jobs])
-        rows = ckpt.rows
-        args = (rows, dy.shape[-1], ckpt.features, len(jobs), js)
-        ws = torch.empty(lib.nf_act8_wgrad_workspace_floats(*args), dtype=torch.float32, device=dev)
-        dw = torch.empty(sum(b * d for _, b, _, d, _ in jobs), dtype=torch.float32, device=dev)
-        db = torch.empty(sum(b for _, b, _, _, e in jobs if e), dtype=torch.float32, device=dev)
-        check(lib.nf_act8_wgrad(_DTYPES[dy.dtype], ptr(m), m.stride(0), dy.shape[-1], ptr(ckpt.codes), ptr(ckpt.scales), ckpt.features, rows, len(jobs), js,
-                                ptr(ws), ptr(dw), ptr(db), _lib.stream()), "nf_act8_wgrad")
+    m = _matrix(dy.detach())
+    js = (_lib.Act8Job * len(jobs))(*[(int(a), int(b), int(c), int(d), int(bool(e))) for a, b, c, d, e in jobs])
+    rows, cols, features = ckpt.rows, dy.shape[-1], ckpt.features
+    n_dw, n_db = sum(b * d for _, b, _, d, _ in jobs), sum(b for _, b, _, _, e in jobs if e)
+    n_ws = lib.nf_act8_wgrad_workspace_floats(rows, cols, features, len(jobs), js)
+    ws = torch.empty(n_ws, dtype=torch.float32, device=dy.device) if n_ws else None
+    both = torch.empty(n_dw + n_db, dtype=torch.float32, device=dy.device)
+    dw, db = both[:n_dw], both[n_dw:]
+    check(lib.nf_act8_wgrad(_DTYPES[dy.dtype], m.data_ptr(), m.stride(0), cols, ckpt.codes.data_ptr(), ckpt.scales.data_ptr(), features, rows, len(jobs), js,
+                            ptr(ws), dw.data_ptr(), db.data_ptr(), _lib.raw_stream(dy)), "nf_act8_wgrad")
     out, o, q = [], 0, 0
     for _, b, _, d, e in jobs:
         out.append((dw[o:o + b * d].view(b, d), db[q:q + b] if e else None))

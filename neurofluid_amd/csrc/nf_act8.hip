@@ -90,34 +90,34 @@ __global__ void __launch_bounds__(256) k_act8_pack(const T* __restrict__ x, long
     }
 }
 
+// A thread writes 16 bytes, next to its neighbours' (8 features of 16 bits, 4 of 32: with 8 of 32 a store's lanes lie 32 bytes apart, 240 us
+// for 63 001 x 2 432 instead of 150).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K, int Kp, int Rp,
                                                      T* __restrict__ out, long long os)
 {
-    const int c = blockIdx.x * 128 + (threadIdx.x & 15) * 8, r0 = blockIdx.y * A8_ROWS;
+    constexpr int PER = 16 / sizeof(T), LANES = 128 / PER;
+    const int c = blockIdx.x * 128 + (threadIdx.x % LANES) * PER, r0 = blockIdx.y * A8_ROWS;
     if (c >= K) return;
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        const int r = r0 + it * 16 + (threadIdx.x >> 4);
+    for (int it = 0; it < A8_ROWS * LANES / 256; ++it) {
+        const int r = r0 + it * (256 / LANES) + threadIdx.x / LANES;
         if (r >= rows) break;
-        const int2 w = *(const int2*)(codes + (long long)r * Kp + c);
+        unsigned w[PER / 4];
+        if (PER == 8) *(uint2*)w = *(const uint2*)(codes + (long long)r * Kp + c);
+        else w[0] = *(const unsigned*)(codes + (long long)r * Kp + c);
         const float s = __uint_as_float((unsigned)scales[(long long)(c >> 5) * Rp + r] << 23);
-        float v[8];
-        f32x2 p;
-        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false); v[0] = p.x * s; v[1] = p.y * s;
-        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true); v[2] = p.x * s; v[3] = p.y * s;
-        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false); v[4] = p.x * s; v[5] = p.y * s;
-        p = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true); v[6] = p.x * s; v[7] = p.y * s;
+        alignas(16) T e[PER];
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i) {
+            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+            a8_st(&e[4 * i], a.x * s); a8_st(&e[4 * i + 1], a.y * s); a8_st(&e[4 * i + 2], b.x * s); a8_st(&e[4 * i + 3], b.y * s);
+        }
         T* o = out + (long long)r * os + c;
-        alignas(16) T e[8];
+        if (VEC && K - c >= PER) *(uint4*)o = *(const uint4*)e;
+        else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a8_st(&e[i], v[i]);
-        if (VEC && K - c >= 8) {
-            ((uint4*)o)[0] = *(const uint4*)e;
-            if (sizeof(T) == 4) ((uint4*)o)[1] = *(const uint4*)(e + 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < PER; ++i)
                 if (c + i < K) o[i] = e[i];
         }
     }
@@ -204,25 +204,28 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 // bf16 matrix instructions with fp32 accumulation give every product exactly, at 16 / 8 / 5.3 times the fp32 matrix rate: the result is that
 // of an fp32 product of dy with the unpacked values, up to the order of the sums.
 //
-// Both operands lie along the outputs, and the reduction runs over the rows: a thread loads 8 rows of 4 (dy) or TK / 32 (codes) adjacent columns, and
-// 8 rows of one column are the 16 bytes that a lane feeds the matrix instruction: the transposition happens in the packing.  A lane's
-// columns go to LDS places 32 apart (column c of quad q at 32 c + q), so that both the writes and the reads run through whole bank rows; which
-// column a matrix row stands for is then settled where the result is stored.
+// Both operands lie along the outputs, and the reduction runs over the rows: a wave loads 8 rows, a lane C adjacent columns of them, and 8 rows of
+// one column are the 16 bytes that a lane feeds the matrix instruction: the transposition happens in the packing.  Column j of lane p goes to
+// LDS place 64 j + p, so that both the writes and the reads run through whole bank rows; which column a matrix row stands for is then settled
+// where the result is stored.
 //
-// Tile: 128 outputs of dy x TK features a workgroup, each of 4 waves a quarter; 64 rows a slab.  The rows are split into slices,
-// whose partial tiles a second launch adds in a fixed order.
+// Tile: (64 C) x (64 C) outputs a workgroup, each of 4 waves a quarter, 32 rows a slab, two slabs in LDS: while one is multiplied the next is
+// packed into the other and the one after that is on its way in registers; one barrier a slab.  C = 4 (256 x 256: 64 matrix instructions a
+// slab and plane for 32 fragment reads) where that fills the chip, else C = 2 (two workgroups a CU).  The rows are split into slices, whose
+// partial tiles a second launch adds in a fixed order.
 // ------------------------------------------------------------------------------------------------
-#define A8_TM 128
 #define A8_MAX_JOBS 16
+#define A8_SLAB 32
 
-struct A8Job { long long out; int dy_col, M, x_col, K, ldo, db, tile0, tiles_k; };     // db: offset of the column sums in the bias blob, -1: none
+struct A8Job { long long out; int dy_col, M, x_col, K, db, tile0, tiles_k; };     // db: offset of the column sums in the slice's record, -1: none
 struct A8Jobs { int n, ntiles; A8Job j[A8_MAX_JOBS]; };
 
 struct A8Args {
     const void* dy; long long dys; const uint8_t* codes; const uint8_t* scales;
     int rows, Kp, Rp, rows_per_slice, nslices;
-    float* out; float* bias;               // slice s at out + s * out_total, bias + s * bias_total
-    long long out_total, bias_total;
+    float* out;                            // slice s at out + s * total: the jobs' tiles, then their column sums
+    float* bias;                           // the same for one slice: the column sums go here
+    long long total;
 };
 
 template <typename T> struct A8Planes { static constexpr int n = 3; };
@@ -238,206 +241,224 @@ __device__ __forceinline__ float a8_rest(float v)
 // the upper halves of two words: (low: a, high: b)
 __device__ __forceinline__ unsigned a8_hi2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 
-template <typename T, int TK, bool VEC>
-__global__ void __launch_bounds__(256, 2) k_act8_wgrad(A8Args a, A8Jobs J)
+template <typename T, int C, bool VEC>
+__global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8Jobs J)
 {
-    constexpr int NP = A8Planes<T>::n, CK = TK / 32;        // CK: adjacent features a thread stages
-    __shared__ uint4 sA[NP][8][A8_TM];
-    __shared__ uint4 sB[8][TK];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave & 1, wk = wave >> 1;
-    const int slice = blockIdx.x / J.ntiles, tile = blockIdx.x - slice * J.ntiles;
+    constexpr int NP = A8Planes<T>::n, TILE = 64 * C, NB = C;        // NB: 32-blocks of a wave in either direction
+    __shared__ uint4 sA[2][NP][4][TILE];
+    __shared__ uint4 sB[2][4][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wk = wave >> 1;
+    // consecutive tiles of a slice share operand columns: they go to one XCD (workgroups go round the eight of them)
+    int id = blockIdx.x;
+    {
+        const int n = gridDim.x, x = id & 7, q = n >> 3, rem = n & 7;
+        id = x * q + min(x, rem) + (id >> 3);
+    }
+    const int slice = id / J.ntiles, tile = id - slice * J.ntiles;
     int ji = 0;
     while (ji + 1 < J.n && tile >= J.j[ji + 1].tile0) ++ji;
     const A8Job job = J.j[ji];
     const int tm = (tile - job.tile0) / job.tiles_k, tk = (tile - job.tile0) - tm * job.tiles_k;
-    const int m0 = tm * A8_TM, k0 = tk * TK;
+    const int m0 = tm * TILE, k0 = tk * TILE;
     const int rb = slice * a.rows_per_slice, re = min(a.rows, rb + a.rows_per_slice);
-    const int q = tid & 31, oct = tid >> 5;
-    // columns of this thread; beyond the job's they are read from inside it (the results are not stored)
-    const int cm = m0 + 4 * q, ck = k0 + CK * q;
-    const int ckl = min(ck, (job.K + 31) / 32 * 32 - CK);
+    // columns of this lane; beyond the job's they are read from inside it (the results are not stored)
+    const int cm = m0 + C * lane, ckl = min(k0 + C * lane, (job.K + 31) / 32 * 32 - C);
+    const bool with_bias = job.db >= 0 && tk == 0, vec = VEC && job.dy_col % C == 0;
+    const bool inside = vec && cm + C <= job.M;
     const T* dyp = (const T*)a.dy + job.dy_col;
     const uint8_t* xp = a.codes + job.x_col + ckl;
     const uint8_t* sp = a.scales + (long long)((job.x_col + ckl) >> 5) * a.Rp;
-    f32x16 acc[2][CK / 2];
+    f32x16 acc[NB][NB];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < CK / 2; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    float bsum[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool with_bias = job.db >= 0 && tk == 0, vec = VEC && job.dy_col % 4 == 0;
+    float bsum[C] = {};
 
-    alignas(16) T dv[8][4];
-    unsigned xv[8][CK / 4];
+    struct alignas(sizeof(T) * C) Row { T v[C]; };
+    Row dv[8];
+    unsigned xv[8];
     uint2 sv;
     auto fetch = [&](int r0) {
-        const int r = r0 + 8 * oct;
+        const int r = r0 + 8 * wave;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const long long rr = min(r + i, re - 1);
             const T* p = dyp + rr * a.dys;
-            if (vec && cm + 4 <= job.M) {
-                if (sizeof(T) == 4) *(uint4*)dv[i] = *(const uint4*)(p + cm);
-                else *(uint2*)dv[i] = *(const uint2*)(p + cm);
-            } else {
+            if (inside) dv[i] = *(const Row*)(p + cm);
+            else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) dv[i][c] = p[min(cm + c, job.M - 1)];
+                for (int c = 0; c < C; ++c) dv[i].v[c] = p[min(cm + c, job.M - 1)];
             }
-            if (CK == 8) { const uint2 v = *(const uint2*)(xp + rr * a.Kp); xv[i][0] = v.x; xv[i][CK / 4 - 1] = v.y; }
-            else xv[i][0] = *(const unsigned*)(xp + rr * a.Kp);
+            if (C == 4) xv[i] = *(const unsigned*)(xp + rr * a.Kp);
+            else xv[i] = *(const unsigned short*)(xp + rr * a.Kp);
         }
-        sv = *(const uint2*)(sp + r);            // (rows are padded to whole slabs)
+        sv = *(const uint2*)(sp + r);            // (rows are padded to 64)
     };
-    if (rb < re) fetch(rb);
-    for (int r0 = rb; r0 < re; r0 += A8_ROWS) {
-        const int left = re - (r0 + 8 * oct);    // rows of this thread's eight that exist
+    auto stage = [&](int r0, int buf) {
+        const int left = re - (r0 + 8 * wave);   // (uniform) rows of this wave's eight that exist
         // dy: planes of the eight rows of each column
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < C; ++c) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = a8_cv(dv[i][c]);
+            for (int i = 0; i < 8; ++i) v[i] = a8_cv(dv[i].v[c]);
             if (left < 8)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.f;
             if (with_bias) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
-                sA[p][oct][32 * c + q] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
+                sA[buf][p][wave][64 * c + lane] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
                 if (p + 1 < NP)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
             }
         }
         // codes: two adjacent features a conversion, then rows paired
-        {
-            float s[8];
+        float s[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? sv.x >> (8 * i) : sv.y >> (8 * i - 32)) & 0xffu) << 23);
-            if (left < 8)
+        for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? sv.x >> (8 * i) : sv.y >> (8 * i - 32)) & 0xffu) << 23);
+        if (left < 8)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i) xv[i] = i < left ? xv[i] : 0u;
 #pragma unroll
-                    for (int w = 0; w < CK / 4; ++w) xv[i][w] = i < left ? xv[i][w] : 0u;
+        for (int h = 0; h < C / 2; ++h) {
+            unsigned e[8];
 #pragma unroll
-            for (int w = 0; w < CK / 4; ++w) {
-                unsigned lo[8], hi[8];           // features (0, 1) and (2, 3) of the word as bf16 pairs
+            for (int i = 0; i < 8; ++i)
+                e[i] = h ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i], s[i], true))
+                         : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i], s[i], false));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    lo[i] = __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i][w], s[i], false));
-                    hi[i] = __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i][w], s[i], true));
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const unsigned* e = c < 2 ? lo : hi;
-                    const unsigned sel = (c & 1) ? 0x07060302u : 0x05040100u;
-                    sB[oct][32 * (4 * w + c) + q] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
-                                                               __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
-                }
+            for (int c = 0; c < 2; ++c) {
+                const unsigned sel = c ? 0x07060302u : 0x05040100u;
+                sB[buf][wave][64 * (2 * h + c) + lane] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
+                                                                    __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
             }
         }
-        if (r0 + A8_ROWS < re) fetch(r0 + A8_ROWS);      // on its way behind the products
-        __syncthreads();
+    };
+    auto multiply = [&](int buf) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
+        for (int ks = 0; ks < 2; ++ks) {
             const int o = 2 * ks + (lane >> 5), l = lane & 31;
-            bf16x8 fb[CK / 2];
+            bf16x8 fb[NB];
 #pragma unroll
-            for (int j = 0; j < CK / 2; ++j) fb[j] = __builtin_bit_cast(bf16x8, sB[o][32 * (wk * (CK / 2) + j) + l]);
+            for (int j = 0; j < NB; ++j) fb[j] = __builtin_bit_cast(bf16x8, sB[buf][o][32 * (wk * NB + j) + l]);
 #pragma unroll
             for (int p = NP - 1; p >= 0; --p)            // the small parts first
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bf16x8 fa = __builtin_bit_cast(bf16x8, sA[p][o][32 * (2 * wm + i) + l]);
+                for (int i = 0; i < NB; ++i) {
+                    const bf16x8 fa = __builtin_bit_cast(bf16x8, sA[buf][p][o][32 * (wm * NB + i) + l]);
 #pragma unroll
-                    for (int j = 0; j < CK / 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
                 }
         }
+    };
+    if (rb < re) {
+        fetch(rb);
+        stage(rb, 0);
+        if (rb + A8_SLAB < re) fetch(rb + A8_SLAB);
         __syncthreads();
+        int buf = 0;
+        for (int r0 = rb; r0 < re; r0 += A8_SLAB, buf ^= 1) {
+            if (r0 + A8_SLAB < re) {
+                stage(r0 + A8_SLAB, buf ^ 1);
+                if (r0 + 2 * A8_SLAB < re) fetch(r0 + 2 * A8_SLAB);
+            }
+            multiply(buf);
+            __syncthreads();
+        }
     }
-    // matrix row i of block b is output 4 i + b of the tile, matrix column j of block b feature CK j + b
-    float* out = a.out + slice * a.out_total + job.out;
+    // place 32 b + i of a tile is column C (32 (b % 2) + i) + b / 2
+    float* out = a.out + slice * a.total + job.out;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int m = m0 + 4 * ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + 2 * wm + i;
-            const int k = k0 + CK * (lane & 31) + wk * (CK / 2);
-            if (m < job.M) {
-                float* o = out + (long long)m * job.ldo + k;
+        for (int j = 0; j < NB; ++j) {
+            const int bm = wm * NB + i, bk = wk * NB + j;
+            const int k = k0 + C * (32 * (bk & 1) + (lane & 31)) + (bk >> 1);
 #pragma unroll
-                for (int j = 0; j < CK / 2; ++j)
-                    if (k + j < job.K) o[j] = acc[i][j][r];
+            for (int r = 0; r < 16; ++r) {
+                const int m = m0 + C * (32 * (bm & 1) + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + (bm >> 1);
+                if (m < job.M && k < job.K) out[(long long)m * job.K + k] = acc[i][j][r];
             }
         }
     if (with_bias) {
-        float* sb = (float*)&sB[0][0];
+        float* sb = (float*)&sB[0][0][0];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sb[oct * A8_TM + 4 * q + c] = bsum[c];
+        for (int c = 0; c < C; ++c) sb[wave * TILE + C * lane + c] = bsum[c];
         __syncthreads();
-        if (tid < A8_TM && m0 + tid < job.M) {
-            float s = 0.f;
+        for (int c = tid; c < TILE && m0 + c < job.M; c += 256)
+            a.bias[slice * a.total + job.db + m0 + c] = (sb[c] + sb[TILE + c]) + (sb[2 * TILE + c] + sb[3 * TILE + c]);
+    }
+}
+
+// Slices added in a fixed order: a thread a quarter of them for four numbers, then the four quarters.  Record: [weights (n_w) | biases].
+__global__ void __launch_bounds__(256) k_act8_fold(const float* __restrict__ part, long long n, long long n_w, long long n_all, int nslices, float* __restrict__ dw,
+                                                   float* __restrict__ db)
+{
+    __shared__ float4 s4[3][64];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const long long i = ((long long)blockIdx.x * 64 + c) * 4;
+    const int per = (nslices + 3) / 4, s0 = g * per, s1 = min(nslices, s0 + per);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < n) {
+#pragma unroll 8
+        for (int s = s0; s < s1; ++s) {
+            const float4 e = *(const float4*)(part + s * n + i);        // (records are whole quads long)
+            v.x += e.x; v.y += e.y; v.z += e.z; v.w += e.w;
+        }
+    }
+    if (g > 0) s4[g - 1][c] = v;
+    __syncthreads();
+    if (g == 0 && i < n) {
+        const float4 b = s4[0][c], d = s4[1][c], e = s4[2][c];
+        const float o[4] = {(v.x + b.x) + (d.x + e.x), (v.y + b.y) + (d.y + e.y), (v.z + b.z) + (d.z + e.z), (v.w + b.w) + (d.w + e.w)};
 #pragma unroll
-            for (int o = 0; o < 8; ++o) s += sb[o * A8_TM + tid];
-            a.bias[slice * a.bias_total + job.db + m0 + tid] = s;
+        for (int k = 0; k < 4; ++k) {
+            if (i + k < n_w) dw[i + k] = o[k];
+            else if (i + k < n_all) db[i + k - n_w] = o[k];
         }
     }
 }
 
-// Slices added in a fixed order: a thread a quarter of them, then the four quarters.
-__global__ void __launch_bounds__(256) k_act8_fold(const float* __restrict__ part, long long n, int nslices, float* __restrict__ out)
-{
-    __shared__ float s4[4][64];
-    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const long long i = (long long)blockIdx.x * 64 + c;
-    const int per = (nslices + 3) / 4, s0 = g * per, s1 = min(nslices, s0 + per);
-    float v = 0.f;
-    if (i < n) {
-#pragma unroll 8
-        for (int s = s0; s < s1; ++s) v += part[s * n + i];
-    }
-    s4[g][c] = v;
-    __syncthreads();
-    if (g == 0 && i < n) out[i] = (s4[0][c] + s4[1][c]) + (s4[2][c] + s4[3][c]);
-}
+struct A8Plan { A8Jobs J; int C, nslices, rows_per_slice; long long n_w, n_b, record; };
 
-static int a8_plan(int njobs, const nf_act8_job_t* jobs, int TK, A8Jobs* J, long long* out_total, long long* bias_total)
+static void a8_tiles(int njobs, const nf_act8_job_t* jobs, int C, A8Plan* p)
 {
+    const int tile = 64 * C;
     int tiles = 0;
     long long out = 0, bias = 0;
     for (int i = 0; i < njobs; ++i) {
         const nf_act8_job_t& s = jobs[i];
-        A8Job& j = J->j[i];
-        j.dy_col = s.dy_col; j.M = s.M; j.x_col = s.x_col; j.K = s.K; j.ldo = s.K; j.out = out;
+        A8Job& j = p->J.j[i];
+        j.dy_col = s.dy_col; j.M = s.M; j.x_col = s.x_col; j.K = s.K; j.out = out;
         j.db = s.bias ? (int)bias : -1;
-        j.tile0 = tiles; j.tiles_k = (s.K + TK - 1) / TK;
-        tiles += ((s.M + A8_TM - 1) / A8_TM) * j.tiles_k;
+        j.tile0 = tiles; j.tiles_k = (s.K + tile - 1) / tile;
+        tiles += ((s.M + tile - 1) / tile) * j.tiles_k;
         out += (long long)s.M * s.K;
         if (s.bias) bias += s.M;
     }
-    J->n = njobs; J->ntiles = tiles;
-    *out_total = out; *bias_total = bias;
-    return tiles;
+    p->J.n = njobs; p->J.ntiles = tiles; p->C = C;
+    p->n_w = out; p->n_b = bias; p->record = (out + bias + 3) / 4 * 4;
 }
 
-// The tile's width: 256 features halve the reads of dy; 128 where no job has more.
-static int a8_tk(int njobs, const nf_act8_job_t* jobs)
+static A8Plan a8_plan(int rows, int njobs, const nf_act8_job_t* jobs)
 {
-    for (int i = 0; i < njobs; ++i)
-        if (jobs[i].K > 128) return 256;
-    return 128;
-}
-
-static int a8_slices(int rows, int tiles)
-{
-    const int slabs = (rows + A8_ROWS - 1) / A8_ROWS;
-    int s = 512 / (tiles > 0 ? tiles : 1);
-    if (s > slabs / 4) s = slabs / 4;
+    A8Plan p;
+    const int slabs = (rows + A8_SLAB - 1) / A8_SLAB;
+    a8_tiles(njobs, jobs, 4, &p);
+    int want = 256;
+    if (p.J.ntiles < 32) { a8_tiles(njobs, jobs, 2, &p); want = 512; }
+    int s = want / p.J.ntiles;
+    if (s > slabs / 8) s = slabs / 8;
     if (s < 1) s = 1;
     const int per = (slabs + s - 1) / s;
-    return per > 0 ? (slabs + per - 1) / per : 1;
+    p.nslices = per > 0 ? (slabs + per - 1) / per : 1;
+    p.rows_per_slice = per * A8_SLAB;
+    return p;
 }
 
 static int a8_jobs_ok(const char* who, int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs)
@@ -458,11 +479,8 @@ static int a8_jobs_ok(const char* who, int rows, int dy_cols, int x_cols, int nj
 extern "C" size_t nf_act8_wgrad_workspace_floats(int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs)
 {
     if (a8_jobs_ok(__func__, rows, dy_cols, x_cols, njobs, jobs)) return 0;
-    A8Jobs J;
-    long long o, b;
-    const int tiles = a8_plan(njobs, jobs, a8_tk(njobs, jobs), &J, &o, &b);
-    const int ns = a8_slices(rows, tiles);
-    return ns > 1 ? (size_t)ns * (size_t)(o + b) : 0;
+    const A8Plan p = a8_plan(rows, njobs, jobs);
+    return p.nslices > 1 ? (size_t)p.nslices * (size_t)p.record : 0;
 }
 
 extern "C" int nf_act8_wgrad(int dtype, const void* dy, int64_t dy_stride, int dy_cols, const uint8_t* codes, const uint8_t* scales, int x_cols, int rows,
@@ -471,43 +489,36 @@ extern "C" int nf_act8_wgrad(int dtype, const void* dy, int64_t dy_stride, int d
     NF_CHECK_ARG(dtype >= 0 && dtype <= 2, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
     const int rc = a8_jobs_ok(__func__, rows, dy_cols, x_cols, njobs, jobs);
     if (rc) return rc;
-    A8Jobs J;
+    const A8Plan p = a8_plan(rows, njobs, jobs);
+    NF_CHECK_ARG(dweights && (p.n_b == 0 || dbias) && (rows == 0 || (dy && codes && scales)), "null pointer");
+    NF_CHECK_ARG(p.nslices == 1 || (workspace && (uintptr_t)workspace % 16 == 0), "null or unaligned workspace (nf_act8_wgrad_workspace_floats)");
+    NF_CHECK_ARG((long long)p.nslices * p.J.ntiles <= 0x7fffffffLL && p.record / 256 < 0x7fffffffLL, "too many tiles");
     A8Args a = {};
-    const int TK = a8_tk(njobs, jobs);
-    const int tiles = a8_plan(njobs, jobs, TK, &J, &a.out_total, &a.bias_total);
-    NF_CHECK_ARG(dweights && (a.bias_total == 0 || dbias) && (rows == 0 || (dy && codes && scales)), "null pointer");
-    const int ns = a8_slices(rows, tiles);
-    NF_CHECK_ARG(ns == 1 || workspace, "null workspace (nf_act8_wgrad_workspace_floats)");
-    NF_CHECK_ARG((long long)ns * tiles <= 0x7fffffffLL, "too many tiles");
-    const int slabs = (rows + A8_ROWS - 1) / A8_ROWS;
     a.dy = dy; a.dys = dy_stride; a.codes = codes; a.scales = scales;
-    a.rows = rows; a.Kp = (int)a8_kp(x_cols); a.Rp = (int)a8_rp(rows); a.nslices = ns;
-    a.rows_per_slice = (slabs + ns - 1) / ns * A8_ROWS;
-    a.out = ns > 1 ? workspace : dweights;
-    a.bias = ns > 1 ? workspace + (size_t)ns * a.out_total : dbias;
+    a.rows = rows; a.Kp = (int)a8_kp(x_cols); a.Rp = (int)a8_rp(rows); a.nslices = p.nslices; a.rows_per_slice = p.rows_per_slice;
+    a.total = p.record;
+    a.out = p.nslices > 1 ? workspace : dweights;
+    a.bias = p.nslices > 1 ? workspace + p.n_w : dbias;
     const int es = dtype == 0 ? 4 : 2;
-    const bool vec = (uintptr_t)dy % (4 * es) == 0 && dy_stride % 4 == 0;
-    const dim3 grid((unsigned)(ns * tiles));
+    const bool vec = (uintptr_t)dy % (p.C * es) == 0 && dy_stride % p.C == 0;
+    const dim3 grid((unsigned)(p.nslices * p.J.ntiles));
     hipStream_t st = (hipStream_t)stream;
-#define A8_GO(T, K_)                                                                                       \
+#define A8_GO(T, C_)                                                                                       \
     do {                                                                                                   \
-        if (vec) hipLaunchKernelGGL((k_act8_wgrad<T, K_, true>), grid, dim3(256), 0, st, a, J);             \
-        else hipLaunchKernelGGL((k_act8_wgrad<T, K_, false>), grid, dim3(256), 0, st, a, J);                \
+        if (vec) hipLaunchKernelGGL((k_act8_wgrad<T, C_, true>), grid, dim3(256), 0, st, a, p.J);           \
+        else hipLaunchKernelGGL((k_act8_wgrad<T, C_, false>), grid, dim3(256), 0, st, a, p.J);              \
     } while (0)
-#define A8_GO_K(T) do { if (TK == 256) A8_GO(T, 256); else A8_GO(T, 128); } while (0)
-    if (dtype == 0) A8_GO_K(float);
-    else if (dtype == 1) A8_GO_K(A8Bf16);
-    else A8_GO_K(A8F16);
-#undef A8_GO_K
+#define A8_GO_C(T) do { if (p.C == 4) A8_GO(T, 4); else A8_GO(T, 2); } while (0)
+    if (dtype == 0) A8_GO_C(float);
+    else if (dtype == 1) A8_GO_C(A8Bf16);
+    else A8_GO_C(A8F16);
+#undef A8_GO_C
 #undef A8_GO
     NF_CHECK_LAUNCH();
-    if (ns > 1) {
-        hipLaunchKernelGGL(k_act8_fold, dim3((unsigned)((a.out_total + 63) / 64)), dim3(256), 0, st, (const float*)a.out, a.out_total, ns, dweights);
+    if (p.nslices > 1) {
+        hipLaunchKernelGGL(k_act8_fold, dim3((unsigned)((p.record + 255) / 256)), dim3(256), 0, st, (const float*)workspace, p.record, p.n_w, p.n_w + p.n_b, p.nslices,
+                           dweights, p.n_b ? dbias : nullptr);
         NF_CHECK_LAUNCH();
-        if (a.bias_total) {
-            hipLaunchKernelGGL(k_act8_fold, dim3((unsigned)((a.bias_total + 63) / 64)), dim3(256), 0, st, (const float*)a.bias, a.bias_total, ns, dbias);
-            NF_CHECK_LAUNCH();
-        }
     }
     return NF_OK;
 }

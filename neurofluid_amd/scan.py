@@ -29,7 +29,7 @@ def _check(gate, x, what):
         raise TypeError(f"{what}: x must be float32, bfloat16 or float16, not {x.dtype}")
     if gate.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"{what}: the gate must have x's dtype or float32, not {gate.dtype}")
-    if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] not in (1, x.shape[-1]):
+    if gate.shape != x.shape and (gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] != 1):
         raise ValueError(f"{what}: gate {tuple(gate.shape)} does not fit x {tuple(x.shape)} (same shape, or one gate a step: last axis 1)")
     if x.shape[-1] < 1:
         raise ValueError(f"{what}: x has no channels")
@@ -38,7 +38,7 @@ def _check(gate, x, what):
 
 
 def _check_state(t, shape, x, what, name):
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != x.device:
+    if t.dtype is not torch.float32 or t.shape != shape or t.device != x.device:
         raise ValueError(f"{what}: {name} must be float32 {shape} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
@@ -56,74 +56,78 @@ def _describe(gate, x, row_splits, log_gate, reverse):
 
 
 def _workspace(lib, s, backward, dev):
-    s.workspace_bytes = lib.nf_scan_workspace_bytes(ctypes.byref(s), backward)
+    s.workspace_bytes = lib.nf_scan_workspace_bytes(s, backward)
     ws = torch.empty(s.workspace_bytes, dtype=torch.uint8, device=dev) if s.workspace_bytes else None
     s.workspace = ptr(ws)
     return ws
 
 
+@_lib.on_device
+def _forward(x, gate, h0, row_splits, log_gate, reverse, keep):
+    """-> h, h_last and what the backward needs besides the inputs: (states, sid, plan)."""
+    lib = _lib.load()
+    dev = x.device
+    s = _describe(gate, x, row_splits, log_gate, reverse)
+    n_state = s.n_seq if row_splits is not None else s.B
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if s.B == 0 or (s.T == 0 and row_splits is None):
+        last = torch.zeros(n_state, s.D, dtype=torch.float32, device=dev) if h0 is None else h0.clone()
+        return h, last, (None, None, (0, 0, 0))
+    last = torch.empty(n_state, s.D, dtype=torch.float32, device=dev)
+    n_states = ctypes.c_size_t()
+    check(lib.nf_scan_plan(s, n_states), "nf_scan_plan")
+    states = torch.empty(n_states.value, dtype=torch.float32, device=dev) if keep else None
+    sid = torch.empty(s.T, dtype=torch.int32, device=dev) if row_splits is not None else None
+    s.h0, s.h, s.h_last, s.states, s.sid = ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(sid)
+    ws = _workspace(lib, s, 0, dev)              # noqa: F841  (alive until the launches are enqueued)
+    check(lib.nf_scan_fwd(s, _lib.raw_stream(x)), "nf_scan_fwd")
+    return h, last, (states, sid, (s.vec, s.cg, s.mode))
+
+
 class _ScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, row_splits, log_gate, reverse):
-        lib = _lib.load()
-        dev = x.device
         ctx.set_materialize_grads(False)
-        g_, x_ = _rows(gate.detach()), _rows(x.detach())
-        h0_ = None if h0 is None else h0.detach().contiguous()
-        need = any(ctx.needs_input_grad[:3])
-        with torch.cuda.device(dev):
-            s = _describe(g_, x_, row_splits, log_gate, reverse)
-            n_state = s.n_seq if row_splits is not None else s.B
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            last = torch.empty(n_state, s.D, dtype=torch.float32, device=dev)
-            states = sid = None
-            if s.T == 0 and row_splits is None:
-                last = torch.zeros_like(last) if h0_ is None else h0_.clone()
-            elif s.B > 0:
-                n_states = ctypes.c_size_t()
-                check(lib.nf_scan_plan(ctypes.byref(s), ctypes.byref(n_states)), "nf_scan_plan")
-                states = torch.empty(n_states.value, dtype=torch.float32, device=dev) if need else None
-                sid = torch.empty(s.T, dtype=torch.int32, device=dev) if row_splits is not None else None
-                s.h0, s.h, s.h_last, s.states, s.sid = ptr(h0_), ptr(h), ptr(last), ptr(states), ptr(sid)
-                ws = _workspace(lib, s, 0, dev)              # noqa: F841  (alive until the launches are enqueued)
-                check(lib.nf_scan_fwd(ctypes.byref(s), _lib.stream()), "nf_scan_fwd")
-        if need:
-            ctx.save_for_backward(gate, x, h0, row_splits, states, sid)
-            ctx.opts, ctx.plan = (log_gate, reverse), (s.vec, s.cg, s.mode)
+        h, last, (states, sid, plan) = _forward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(),
+                                                row_splits, log_gate, reverse, True)
+        ctx.save_for_backward(gate, x, h0, row_splits, states, sid)
+        ctx.opts, ctx.plan = (log_gate, reverse), plan
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, g_last):
-        lib = _lib.load()
         gate, x, h0, row_splits, states, sid = ctx.saved_tensors
-        dev = x.device
-        g_, x_ = _rows(gate.detach()), _rows(x.detach())
-        h0_ = None if h0 is None else h0.detach().contiguous()
-        gl = None if g_last is None else g_last.detach().contiguous()
-        need = ctx.needs_input_grad
-        with torch.cuda.device(dev):
-            s = _describe(g_, x_, row_splits, *ctx.opts)
-            s.vec, s.cg, s.mode = ctx.plan
-            n_state = s.n_seq if row_splits is not None else s.B
-            dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[0] else None
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[1] else None
-            dh0 = torch.empty(n_state, s.D, dtype=torch.float32, device=dev) if need[2] else None
-            if s.T == 0 and row_splits is None:
-                if dh0 is not None:
-                    dh0.copy_(gl) if gl is not None else dh0.zero_()
-            elif s.B > 0:
-                y = None
-                if g is not None:
-                    y = _rows(g.detach())
-                    if y.data_ptr() % (s.vec * y.element_size()) or any(v % s.vec for v in y.stride()[:-1]):
-                        y = y.clone(memory_format=torch.contiguous_format)
-                    s.g_sb, s.g_st = (0, y.stride(0)) if row_splits is not None else (y.stride(0), y.stride(1))
-                s.g, s.h0, s.g_last, s.states, s.sid = ptr(y), ptr(h0_), ptr(gl), ptr(states), ptr(sid)
-                s.dgate, s.dx, s.dh0 = ptr(dgate), ptr(dx), ptr(dh0)
-                ws = _workspace(lib, s, 1, dev)              # noqa: F841
-                check(lib.nf_scan_bwd(ctypes.byref(s), _lib.stream()), "nf_scan_bwd")
-        return dgate, dx, dh0, None, None, None
+        return _backward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(), row_splits, states, sid, g, g_last,
+                         ctx.opts, ctx.plan, ctx.needs_input_grad) + (None, None, None)
+
+
+@_lib.on_device
+def _backward(x, gate, h0, row_splits, states, sid, g, g_last, opts, plan, need):
+    lib = _lib.load()
+    dev = x.device
+    gl = None if g_last is None else g_last.detach().contiguous()
+    s = _describe(gate, x, row_splits, *opts)
+    s.vec, s.cg, s.mode = plan
+    n_state = s.n_seq if row_splits is not None else s.B
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[0] else None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[1] else None
+    dh0 = torch.empty(n_state, s.D, dtype=torch.float32, device=dev) if need[2] else None
+    if s.B == 0 or (s.T == 0 and row_splits is None):
+        if dh0 is not None:
+            dh0.copy_(gl) if gl is not None else dh0.zero_()
+        return dgate, dx, dh0
+    y = None
+    if g is not None:
+        y = _rows(g.detach())
+        if y.data_ptr() % (s.vec * y.element_size()) or any(v % s.vec for v in y.stride()[:-1]):
+            y = y.clone(memory_format=torch.contiguous_format)
+        s.g_sb, s.g_st = (0, y.stride(0)) if row_splits is not None else (y.stride(0), y.stride(1))
+    s.g, s.h0, s.g_last, s.states, s.sid = ptr(y), ptr(h0), ptr(gl), ptr(states), ptr(sid)
+    s.dgate, s.dx, s.dh0 = ptr(dgate), ptr(dx), ptr(dh0)
+    ws = _workspace(lib, s, 1, dev)              # noqa: F841
+    check(lib.nf_scan_bwd(s, _lib.raw_stream(x)), "nf_scan_bwd")
+    return dgate, dx, dh0
 
 
 def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=None):
@@ -151,7 +155,9 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     if h0 is not None:
         _check_state(h0, (row_splits.numel() - 1 if packed else x.shape[0], x.shape[-1]), x, what, "h0")
     ops._require_cuda(gate, x)
-    return _ScanFn.apply(gate, x, h0, row_splits, bool(log_gate), bool(reverse))
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _ScanFn.apply(gate, x, h0, row_splits, bool(log_gate), bool(reverse))
+    return _forward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(), row_splits, log_gate, reverse, False)[:2]
 
 
 def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
@@ -162,25 +168,30 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
     _check(gate, x, what)
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be (rows, D), got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (gate, x, state)):
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
         raise RuntimeError(f"{what} carries no gradients (use gated_scan, or torch.no_grad())")
-    out = state if out is None else out
-    for t, name in ((state, "state"), (out, "out")):
-        _check_state(t, tuple(x.shape), x, what, name)
-        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    rows, D = x.shape
+    span = []
+    for t, name in ((state, "state"),) if out is None else ((state, "state"), (out, "out")):
+        _check_state(t, x.shape, x, what, name)
+        s0, s1 = t.stride()
+        if (D > 1 and s1 != 1) or (rows > 1 and s0 < D):
             raise ValueError(f"{what}: {name} needs adjacent channels and rows that do not overlap")
-    if out.data_ptr() != state.data_ptr() or out.stride() != state.stride():
-        a0, b0 = state.data_ptr(), out.data_ptr()
-        span = [4 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) if t.numel() else 0 for t in (state, out)]
-        if a0 < b0 + span[1] and b0 < a0 + span[0]:
-            raise ValueError(f"{what}: out overlaps state without being it")
+        span.append((t.data_ptr(), s0, 4 * ((rows - 1) * s0 + D)))
+    (a, sa, na), (b, sb, nb) = span[0], span[-1]
+    if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na:
+        raise ValueError(f"{what}: out overlaps state without being it")
     ops._require_cuda(gate, x)
-    lib = _lib.load()
+    return _step(x, gate, a, sa, b, sb, log_gate)
+
+
+@_lib.on_device
+def _step(x, gate, state, state_stride, out, out_stride, log_gate):
     g_, x_ = _rows(gate), _rows(x)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if h.numel():
-        with torch.cuda.device(x.device):
-            check(lib.nf_scan_step(_DTYPES[x.dtype], int(gate.dtype == torch.float32), int(gate.shape[-1] == 1), int(log_gate), x.shape[0], x.shape[1],
-                                   ptr(g_), g_.stride(0), ptr(x_), x_.stride(0), ptr(state), state.stride(0), ptr(out), out.stride(0), ptr(h),
-                                   _lib.stream()), "nf_scan_step")
+    rows, D = x.shape
+    h = torch.empty((rows, D), dtype=x.dtype, device=x.device)
+    if rows:
+        check(_lib.load().nf_scan_step(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[1] == 1, bool(log_gate), rows, D, g_.data_ptr(),
+                                       g_.stride(0), x_.data_ptr(), x_.stride(0), state, state_stride, out, out_stride, h.data_ptr(),
+                                       _lib.raw_stream(x)), "nf_scan_step")
     return h
