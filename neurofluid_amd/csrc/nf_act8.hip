@@ -216,6 +216,9 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 // ------------------------------------------------------------------------------------------------
 #define A8_MAX_JOBS 16
 #define A8_SLAB 32
+#ifndef A8_VALU
+#define A8_VALU 6
+#endif
 
 struct A8Job { long long out; int dy_col, M, x_col, K, db, tile0, tiles_k; };     // db: offset of the column sums in the slice's record, -1: none
 struct A8Jobs { int n, ntiles; A8Job j[A8_MAX_JOBS]; };
@@ -227,6 +230,8 @@ struct A8Args {
     float* bias;                           // the same for one slice: the column sums go here
     long long total;
 };
+
+template <bool B> struct A8Bool { static constexpr bool value = B; };
 
 template <typename T> struct A8Planes { static constexpr int n = 3; };
 template <> struct A8Planes<A8F16> { static constexpr int n = 2; };
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
     const bool with_bias = job.db >= 0 && tk == 0, vec = VEC && job.dy_col % C == 0;
     const bool inside = vec && cm + C <= job.M;
     const T* dyp = (const T*)a.dy + job.dy_col;
-    const uint8_t* xp = a.codes + job.x_col + ckl;
+    const uint8_t* xp = a.codes + job.x_col;
     const uint8_t* sp = a.scales + (long long)((job.x_col + ckl) >> 5) * a.Rp;
     f32x16 acc[NB][NB];
 #pragma unroll
@@ -278,37 +283,38 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
     float bsum[C] = {};
 
     struct alignas(sizeof(T) * C) Row { T v[C]; };
-    Row dv[8];
-    unsigned xv[8];
-    uint2 sv;
-    auto fetch = [&](int r0) {
+    struct Regs { Row d[8]; unsigned x[8]; uint2 s; };
+    // FULL: the tile lies inside the job and the slab inside the slice, BIAS: the columns of dy are summed (both uniform)
+    auto fetch = [&](Regs& g, int r0, auto full) {
         const int r = r0 + 8 * wave;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const long long rr = min(r + i, re - 1);
             const T* p = dyp + rr * a.dys;
-            if (inside) dv[i] = *(const Row*)(p + cm);
+            if (decltype(full)::value) g.d[i] = *(const Row*)(p + cm);
+            else if (inside) g.d[i] = *(const Row*)(p + cm);
             else {
 #pragma unroll
-                for (int c = 0; c < C; ++c) dv[i].v[c] = p[min(cm + c, job.M - 1)];
+                for (int c = 0; c < C; ++c) g.d[i].v[c] = p[min(cm + c, job.M - 1)];
             }
-            if (C == 4) xv[i] = *(const unsigned*)(xp + rr * a.Kp);
-            else xv[i] = *(const unsigned short*)(xp + rr * a.Kp);
+            if (C == 4) g.x[i] = *(const unsigned*)(xp + rr * a.Kp + ckl);
+            else g.x[i] = *(const unsigned short*)(xp + rr * a.Kp + ckl);
         }
-        sv = *(const uint2*)(sp + r);            // (rows are padded to 64)
+        g.s = *(const uint2*)(sp + min(r, a.Rp - 8));      // (rows are padded to 64)
     };
-    auto stage = [&](int r0, int buf) {
-        const int left = re - (r0 + 8 * wave);   // (uniform) rows of this wave's eight that exist
+    auto stage = [&](Regs& g, int r0, int buf, auto full, auto bias) {
+        const int left = re - (r0 + 8 * wave);   // rows of this wave's eight that exist
+        const bool cut = !decltype(full)::value && left < 8;
         // dy: planes of the eight rows of each column
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = a8_cv(dv[i].v[c]);
-            if (left < 8)
+            for (int i = 0; i < 8; ++i) v[i] = a8_cv(g.d[i].v[c]);
+            if (cut)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.f;
-            if (with_bias) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            if (decltype(bias)::value) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
                 sA[buf][p][wave][64 * c + lane] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
@@ -320,17 +326,17 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         // codes: two adjacent features a conversion, then rows paired
         float s[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? sv.x >> (8 * i) : sv.y >> (8 * i - 32)) & 0xffu) << 23);
-        if (left < 8)
+        for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? g.s.x >> (8 * i) : g.s.y >> (8 * i - 32)) & 0xffu) << 23);
+        if (cut)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) xv[i] = i < left ? xv[i] : 0u;
+            for (int i = 0; i < 8; ++i) g.x[i] = i < left ? g.x[i] : 0u;
 #pragma unroll
         for (int h = 0; h < C / 2; ++h) {
             unsigned e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                e[i] = h ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i], s[i], true))
-                         : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[i], s[i], false));
+                e[i] = h ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(g.x[i], s[i], true))
+                         : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(g.x[i], s[i], false));
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const unsigned sel = c ? 0x07060302u : 0x05040100u;
@@ -356,20 +362,54 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
                 }
         }
     };
-    if (rb < re) {
-        fetch(rb);
-        stage(rb, 0);
-        if (rb + A8_SLAB < re) fetch(rb + A8_SLAB);
+    // Slab n is multiplied while n + 1 is packed from one set of registers and n + 2, n + 3 are on their way (the other set, then the same): a load
+    // has two slabs' time.  In the main loop everything is one basic block, the packing spread between the matrix instructions (a wave issues in
+    // order: without the spread the matrix pipe idles while a wave packs).
+    auto step = [&](Regs& g, int r0, int buf, auto full, auto bias) {
+        stage(g, r0 + A8_SLAB, buf ^ 1, full, bias);
+        fetch(g, r0 + 3 * A8_SLAB, full);
+        multiply(buf);
+        if (decltype(full)::value) {
+#pragma unroll
+            for (int k = 0; k < 2 * NP * NB * NB; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x002, A8_VALU, 0);     // vector instructions
+                __builtin_amdgcn_sched_group_barrier(0x080, 1, 0);           // an LDS access
+            }
+        }
         __syncthreads();
-        int buf = 0;
-        for (int r0 = rb; r0 < re; r0 += A8_SLAB, buf ^= 1) {
+    };
+    auto run = [&](auto whole, auto bias) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        Regs g0, g1;
+        A8Bool<false> part;
+        fetch(g0, rb, part);
+        fetch(g1, rb + A8_SLAB, part);
+        stage(g0, rb, 0, part, bias);
+        fetch(g0, rb + 2 * A8_SLAB, part);
+        __syncthreads();
+        int r0 = rb;
+        if (WHOLE)
+            for (; r0 + 3 * A8_SLAB <= re; r0 += 2 * A8_SLAB) {              // (both packed slabs exist)
+                step(g1, r0, 0, whole, bias);
+                step(g0, r0 + A8_SLAB, 1, whole, bias);
+            }
+        for (int buf = 0; r0 < re; r0 += A8_SLAB, buf ^= 1) {
             if (r0 + A8_SLAB < re) {
-                stage(r0 + A8_SLAB, buf ^ 1);
-                if (r0 + 2 * A8_SLAB < re) fetch(r0 + 2 * A8_SLAB);
+                if (buf) stage(g0, r0 + A8_SLAB, 0, part, bias);
+                else stage(g1, r0 + A8_SLAB, 1, part, bias);
+                if (buf) fetch(g0, r0 + 3 * A8_SLAB, part);
+                else fetch(g1, r0 + 3 * A8_SLAB, part);
             }
             multiply(buf);
             __syncthreads();
         }
+    };
+    if (rb < re) {
+        const bool whole = vec && m0 + TILE <= job.M;
+        if (whole && with_bias) run(A8Bool<true>(), A8Bool<true>());
+        else if (whole) run(A8Bool<true>(), A8Bool<false>());
+        else run(A8Bool<false>(), A8Bool<true>());
     }
     // place 32 b + i of a tile is column C (32 (b % 2) + i) + b / 2
     float* out = a.out + slice * a.total + job.out;
