@@ -216,9 +216,6 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 // ------------------------------------------------------------------------------------------------
 #define A8_MAX_JOBS 16
 #define A8_SLAB 32
-#ifndef A8_VALU
-#define A8_VALU 6
-#endif
 
 struct A8Job { long long out; int dy_col, M, x_col, K, db, tile0, tiles_k; };     // db: offset of the column sums in the slice's record, -1: none
 struct A8Jobs { int n, ntiles; A8Job j[A8_MAX_JOBS]; };
@@ -284,15 +281,14 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
 
     struct alignas(sizeof(T) * C) Row { T v[C]; };
     struct Regs { Row d[8]; unsigned x[8]; uint2 s; };
-    // FULL: the tile lies inside the job and the slab inside the slice, BIAS: the columns of dy are summed (both uniform)
-    auto fetch = [&](Regs& g, int r0, auto full) {
+    // Any slab: rows behind the slice are not read, columns behind the job are read from inside it.
+    auto fetch_part = [&](Regs& g, int r0) {
         const int r = r0 + 8 * wave;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const long long rr = min(r + i, re - 1);
             const T* p = dyp + rr * a.dys;
-            if (decltype(full)::value) g.d[i] = *(const Row*)(p + cm);
-            else if (inside) g.d[i] = *(const Row*)(p + cm);
+            if (inside) g.d[i] = *(const Row*)(p + cm);
             else {
 #pragma unroll
                 for (int c = 0; c < C; ++c) g.d[i].v[c] = p[min(cm + c, job.M - 1)];
@@ -302,106 +298,131 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         }
         g.s = *(const uint2*)(sp + min(r, a.Rp - 8));      // (rows are padded to 64)
     };
-    auto stage = [&](Regs& g, int r0, int buf, auto full, auto bias) {
-        const int left = re - (r0 + 8 * wave);   // rows of this wave's eight that exist
-        const bool cut = !decltype(full)::value && left < 8;
-        // dy: planes of the eight rows of each column
+    // A whole slab of a tile inside its job.  (Behind the slice's last eight rows: those again, never used.)
+    auto fetch_full = [&](Regs& g, int r0) {
+        const int r = min(r0 + 8 * wave, re - 8);
+        const T* p = dyp + r * a.dys;
+        const uint8_t* x = xp + (long long)r * a.Kp;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float v[8];
+        for (int i = 0; i < 8; ++i) { g.d[i] = *(const Row*)(p + (unsigned)cm); p += a.dys; }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = a8_cv(g.d[i].v[c]);
-            if (cut)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.f;
-            if (decltype(bias)::value) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                sA[buf][p][wave][64 * c + lane] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
-                if (p + 1 < NP)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
-            }
+        for (int i = 0; i < 8; ++i) {
+            if (C == 4) g.x[i] = *(const unsigned*)(x + (unsigned)ckl);
+            else g.x[i] = *(const unsigned short*)(x + (unsigned)ckl);
+            x += a.Kp;
         }
-        // codes: two adjacent features a conversion, then rows paired
-        float s[8];
+        g.s = *(const uint2*)(sp + min(r0 + 8 * wave, a.Rp - 8));
+    };
+    // Packing a slab, in C * NP pieces for dy (a column's plane each) and C for the codes (a feature each).
+    constexpr int PIECES = C * NP + C;
+    float v[8];          // what is left of the column
+    unsigned e[8];       // two features as bf16 pairs
+    auto pack = [&](const Regs& g, int buf, int piece, int left, auto full, auto bias) {
+        const bool cut = !decltype(full)::value && left < 8;
+        if (piece < C * NP) {
+            const int c = piece / NP, p = piece % NP;
+            if (NP == 1 && !decltype(bias)::value && !cut) {         // bf16: the halves as they are
+                const unsigned sel = (c & 1) ? 0x07060302u : 0x05040100u;
+                unsigned w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __uint_as_float(((i < 4 ? g.s.x >> (8 * i) : g.s.y >> (8 * i - 32)) & 0xffu) << 23);
-        if (cut)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g.x[i] = i < left ? g.x[i] : 0u;
-#pragma unroll
-        for (int h = 0; h < C / 2; ++h) {
-            unsigned e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                e[i] = h ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(g.x[i], s[i], true))
-                         : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(g.x[i], s[i], false));
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const unsigned sel = c ? 0x07060302u : 0x05040100u;
-                sB[buf][wave][64 * (2 * h + c) + lane] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
-                                                                    __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
+                for (int i = 0; i < 8; ++i) w[i] = ((const unsigned*)g.d[i].v)[c / 2];
+                sA[buf][0][wave][64 * c + lane] = make_uint4(__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+                                                             __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel));
+                return;
             }
+            if (p == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = a8_cv(g.d[i].v[c]);
+                if (cut)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.f;
+                if (decltype(bias)::value) bsum[c] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
+            sA[buf][p][wave][64 * c + lane] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
+            if (p + 1 < NP)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
+        } else {
+            const int f = piece - C * NP;
+            if ((f & 1) == 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float s = __uint_as_float(((i < 4 ? g.s.x >> (8 * i) : g.s.y >> (8 * i - 32)) & 0xffu) << 23);
+                    const unsigned w = cut && i >= left ? 0u : g.x[i];
+                    e[i] = f ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
+                             : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+                }
+            const unsigned sel = (f & 1) ? 0x07060302u : 0x05040100u;
+            sB[buf][wave][64 * f + lane] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
+                                                      __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
         }
     };
-    auto multiply = [&](int buf) {
+    bf16x8 fa[2][NP][NB], fb[2][NB];
+    auto fragments = [&](int ks, int buf) {
+        const int o = 2 * ks + (lane >> 5), l = lane & 31;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const int o = 2 * ks + (lane >> 5), l = lane & 31;
-            bf16x8 fb[NB];
+        for (int j = 0; j < NB; ++j) fb[ks][j] = __builtin_bit_cast(bf16x8, sB[buf][o][32 * (wk * NB + j) + l]);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) fb[j] = __builtin_bit_cast(bf16x8, sB[buf][o][32 * (wk * NB + j) + l]);
+        for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p)            // the small parts first
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    const bf16x8 fa = __builtin_bit_cast(bf16x8, sA[buf][p][o][32 * (wm * NB + i) + l]);
-#pragma unroll
-                    for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
-                }
-        }
+            for (int i = 0; i < NB; ++i) fa[ks][p][i] = __builtin_bit_cast(bf16x8, sA[buf][p][o][32 * (wm * NB + i) + l]);
+    };
+    constexpr int PRODUCTS = 2 * NP * NB * NB;
+    auto product = [&](int n) {          // the small parts first
+        const int j = n % NB, i = n / NB % NB, p = NP - 1 - n / (NB * NB) % NP, ks = n / (NB * NB * NP);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks][p][i], fb[ks][j], acc[i][j], 0, 0, 0);
     };
     // Slab n is multiplied while n + 1 is packed from one set of registers and n + 2, n + 3 are on their way (the other set, then the same): a load
-    // has two slabs' time.  In the main loop everything is one basic block, the packing spread between the matrix instructions (a wave issues in
-    // order: without the spread the matrix pipe idles while a wave packs).
-    auto step = [&](Regs& g, int r0, int buf, auto full, auto bias) {
-        stage(g, r0 + A8_SLAB, buf ^ 1, full, bias);
-        fetch(g, r0 + 3 * A8_SLAB, full);
-        multiply(buf);
-        if (decltype(full)::value) {
+    // has two slabs' time.  A wave issues in order, so the packing goes in pieces between the matrix instructions, in whose shadow it runs, and a
+    // slab's fragments are read at once, up to two halves ahead of their use.
+    auto step = [&](Regs& g, int r0, int buf, auto bias) {
+        fragments(0, buf);
+        fragments(1, buf);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2 * NP * NB * NB; ++k) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // a matrix instruction
-                __builtin_amdgcn_sched_group_barrier(0x002, A8_VALU, 0);     // vector instructions
-                __builtin_amdgcn_sched_group_barrier(0x080, 1, 0);           // an LDS access
-            }
+        for (int q = 0; q <= PIECES; ++q) {
+#pragma unroll
+            for (int n = PRODUCTS * q / (PIECES + 1); n < PRODUCTS * (q + 1) / (PIECES + 1); ++n) product(n);
+            if (q < PIECES) pack(g, buf ^ 1, q, 8, A8Bool<true>(), bias);
+            if (q == PIECES - 1) fetch_full(g, r0 + 3 * A8_SLAB);
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     };
     auto run = [&](auto whole, auto bias) {
-        constexpr bool WHOLE = decltype(whole)::value;
         Regs g0, g1;
-        A8Bool<false> part;
-        fetch(g0, rb, part);
-        fetch(g1, rb + A8_SLAB, part);
-        stage(g0, rb, 0, part, bias);
-        fetch(g0, rb + 2 * A8_SLAB, part);
+        auto pack_part = [&](const Regs& g, int r0, int buf) {
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q) pack(g, buf, q, re - (r0 + 8 * wave), A8Bool<false>(), bias);
+        };
+        fetch_part(g0, rb);
+        fetch_part(g1, rb + A8_SLAB);
+        pack_part(g0, rb, 0);
+        fetch_part(g0, rb + 2 * A8_SLAB);
         __syncthreads();
         int r0 = rb;
-        if (WHOLE)
+        if (decltype(whole)::value) {
             for (; r0 + 3 * A8_SLAB <= re; r0 += 2 * A8_SLAB) {              // (both packed slabs exist)
-                step(g1, r0, 0, whole, bias);
-                step(g0, r0 + A8_SLAB, 1, whole, bias);
+                step(g1, r0, 0, bias);
+                step(g0, r0 + A8_SLAB, 1, bias);
             }
+            fetch_part(g1, r0 + A8_SLAB);
+            fetch_part(g0, r0 + 2 * A8_SLAB);
+        }
+        // what is left: up to three slabs, or the whole slice of a tile that its job does not fill
         for (int buf = 0; r0 < re; r0 += A8_SLAB, buf ^= 1) {
             if (r0 + A8_SLAB < re) {
-                if (buf) stage(g0, r0 + A8_SLAB, 0, part, bias);
-                else stage(g1, r0 + A8_SLAB, 1, part, bias);
-                if (buf) fetch(g0, r0 + 3 * A8_SLAB, part);
-                else fetch(g1, r0 + 3 * A8_SLAB, part);
+                if (buf) pack_part(g0, r0 + A8_SLAB, 0);
+                else pack_part(g1, r0 + A8_SLAB, 1);
+                if (buf) fetch_part(g0, r0 + 3 * A8_SLAB);
+                else fetch_part(g1, r0 + 3 * A8_SLAB);
             }
-            multiply(buf);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                fragments(ks, buf);
+#pragma unroll
+                for (int n = 0; n < PRODUCTS / 2; ++n) product(ks * (PRODUCTS / 2) + n);
+            }
             __syncthreads();
         }
     };
