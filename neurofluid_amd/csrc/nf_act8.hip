@@ -298,23 +298,23 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         }
         g.s = *(const uint2*)(sp + min(r, a.Rp - 8));      // (rows are padded to 64)
     };
-    // A whole slab of a tile inside its job.  (Behind the slice's last eight rows: those again, never used.)
-    auto fetch_full = [&](Regs& g, int r0) {
+    // A whole slab of a tile inside its job, row by row from uniform bases.  (Behind the slice's last eight rows: those again, never used.)
+    const unsigned off_d = (unsigned)cm * sizeof(T), off_x = (unsigned)ckl;
+    const long long step_d = a.dys * (long long)sizeof(T);
+    struct Bases { const char* d; const char* x; };
+    auto bases = [&](int r0) {
         const int r = min(r0 + 8 * wave, re - 8);
-        const T* p = dyp + r * a.dys;
-        const uint8_t* x = xp + (long long)r * a.Kp;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { g.d[i] = *(const Row*)(p + (unsigned)cm); p += a.dys; }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (C == 4) g.x[i] = *(const unsigned*)(x + (unsigned)ckl);
-            else g.x[i] = *(const unsigned short*)(x + (unsigned)ckl);
-            x += a.Kp;
-        }
-        g.s = *(const uint2*)(sp + min(r0 + 8 * wave, a.Rp - 8));
+        return Bases{(const char*)dyp + r * step_d, (const char*)xp + (long long)r * a.Kp};
     };
-    // Packing a slab, in C * NP pieces for dy (a column's plane each) and C for the codes (a feature each).
-    constexpr int PIECES = C * NP + C;
+    auto fetch_row = [&](Regs& g, int i, Bases& p) {
+        g.d[i] = *(const Row*)(p.d + off_d);
+        if (C == 4) g.x[i] = *(const unsigned*)(p.x + off_x);
+        else g.x[i] = *(const unsigned short*)(p.x + off_x);
+        p.d += step_d;
+        p.x += a.Kp;
+    };
+    // Packing a slab, in C * NP pieces for dy (a column's plane each) and 2 C for the codes (four rows of two features, a feature).
+    constexpr int PIECES = C * NP + 2 * C;
     float v[8];          // what is left of the column
     unsigned e[8];       // two features as bf16 pairs
     auto pack = [&](const Regs& g, int buf, int piece, int left, auto full, auto bias) {
@@ -343,18 +343,20 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
         } else {
-            const int f = piece - C * NP;
-            if ((f & 1) == 0)
+            const int h = (piece - C * NP) / 4, f = (piece - C * NP) % 4;
+            if (f < 2) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 4 * f; i < 4 * f + 4; ++i) {
                     const float s = __uint_as_float(((i < 4 ? g.s.x >> (8 * i) : g.s.y >> (8 * i - 32)) & 0xffu) << 23);
                     const unsigned w = cut && i >= left ? 0u : g.x[i];
-                    e[i] = f ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
+                    e[i] = h ? __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
                              : __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
                 }
-            const unsigned sel = (f & 1) ? 0x07060302u : 0x05040100u;
-            sB[buf][wave][64 * f + lane] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
-                                                      __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
+            } else {
+                const unsigned sel = f == 3 ? 0x07060302u : 0x05040100u;
+                sB[buf][wave][64 * (2 * h + f - 2) + lane] = make_uint4(__builtin_amdgcn_perm(e[1], e[0], sel), __builtin_amdgcn_perm(e[3], e[2], sel),
+                                                                        __builtin_amdgcn_perm(e[5], e[4], sel), __builtin_amdgcn_perm(e[7], e[6], sel));
+            }
         }
     };
     bf16x8 fa[2][NP][NB], fb[2][NB];
@@ -373,21 +375,31 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks][p][i], fb[ks][j], acc[i][j], 0, 0, 0);
     };
     // Slab n is multiplied while n + 1 is packed from one set of registers and n + 2, n + 3 are on their way (the other set, then the same): a load
-    // has two slabs' time.  A wave issues in order, so the packing goes in pieces between the matrix instructions, in whose shadow it runs, and a
-    // slab's fragments are read at once, up to two halves ahead of their use.
+    // has two slabs' time.  A wave issues in order, so everything else goes in pieces between the matrix instructions, in whose shadow it runs:
+    // the packing with the slab's first half, the loads with the second, whose fragments were read during the first; the next slab's first
+    // fragments are read during the second half, which is why the barrier lies between the two.
     auto step = [&](Regs& g, int r0, int buf, auto bias) {
-        fragments(0, buf);
         fragments(1, buf);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int q = 0; q <= PIECES; ++q) {
+        for (int q = 0; q < PIECES; ++q) {
 #pragma unroll
-            for (int n = PRODUCTS * q / (PIECES + 1); n < PRODUCTS * (q + 1) / (PIECES + 1); ++n) product(n);
-            if (q < PIECES) pack(g, buf ^ 1, q, 8, A8Bool<true>(), bias);
-            if (q == PIECES - 1) fetch_full(g, r0 + 3 * A8_SLAB);
+            for (int n = PRODUCTS / 2 * q / PIECES; n < PRODUCTS / 2 * (q + 1) / PIECES; ++n) product(n);
+            pack(g, buf ^ 1, q, 8, A8Bool<true>(), bias);
             __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
+        fragments(0, buf ^ 1);
+        Bases p = bases(r0 + 3 * A8_SLAB);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+#pragma unroll
+            for (int n = PRODUCTS / 2 * q / 8; n < PRODUCTS / 2 * (q + 1) / 8; ++n) product(PRODUCTS / 2 + n);
+            fetch_row(g, q, p);
+            if (q == 7) g.s = *(const uint2*)(sp + min(r0 + 3 * A8_SLAB + 8 * wave, a.Rp - 8));
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     auto run = [&](auto whole, auto bias) {
         Regs g0, g1;
@@ -402,6 +414,7 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         __syncthreads();
         int r0 = rb;
         if (decltype(whole)::value) {
+            fragments(0, 0);
             for (; r0 + 3 * A8_SLAB <= re; r0 += 2 * A8_SLAB) {              // (both packed slabs exist)
                 step(g1, r0, 0, bias);
                 step(g0, r0 + A8_SLAB, 1, bias);
