@@ -363,11 +363,11 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
     auto fragments = [&](int ks, int buf) {
         const int o = 2 * ks + (lane >> 5), l = lane & 31;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) fb[ks][j] = __builtin_bit_cast(bf16x8, sB[buf][o][32 * (wk * NB + j) + l]);
+        for (int j = 0; j < NB; ++j) fb[ks][j] = __builtin_bit_cast(bf16x8, sB[buf][o][64 * j + 32 * wk + l]);
 #pragma unroll
         for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) fa[ks][p][i] = __builtin_bit_cast(bf16x8, sA[buf][p][o][32 * (wm * NB + i) + l]);
+            for (int i = 0; i < NB; ++i) fa[ks][p][i] = __builtin_bit_cast(bf16x8, sA[buf][p][o][64 * i + 32 * wm + l]);
     };
     constexpr int PRODUCTS = 2 * NP * NB * NB;
     auto product = [&](int n) {          // the small parts first
@@ -445,18 +445,27 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
         else if (whole) run(A8Bool<true>(), A8Bool<false>());
         else run(A8Bool<false>(), A8Bool<true>());
     }
-    // place 32 b + i of a tile is column C (32 (b % 2) + i) + b / 2
+    // place 64 j + p of a tile is column C p + j: a lane holds C adjacent features of its rows
     float* out = a.out + slice * a.total + job.out;
+    const int k = k0 + C * (32 * wk + (lane & 31));
+    const bool quads = job.K % C == 0 && (uintptr_t)out % (4 * C) == 0;
+    typedef float Out __attribute__((ext_vector_type(C)));
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int bm = wm * NB + i, bk = wk * NB + j;
-            const int k = k0 + C * (32 * (bk & 1) + (lane & 31)) + (bk >> 1);
+        for (int r = 0; r < 16; ++r) {
+            const int m = m0 + C * (32 * wm + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + i;
+            if (m >= job.M || k >= job.K) continue;
+            float* o = out + (long long)m * job.K + k;
+            if (quads) {
+                Out w;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m0 + C * (32 * (bm & 1) + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) + (bm >> 1);
-                if (m < job.M && k < job.K) out[(long long)m * job.K + k] = acc[i][j][r];
+                for (int j = 0; j < NB; ++j) w[j] = acc[i][j][r];
+                *(Out*)o = w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    if (k + j < job.K) o[j] = acc[i][j][r];
             }
         }
     if (with_bias) {
