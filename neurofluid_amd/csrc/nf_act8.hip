@@ -91,10 +91,10 @@ __global__ void __launch_bounds__(256) k_act8_pack(const T* __restrict__ x, long
 }
 
 // A thread writes 16 bytes, next to its neighbours' (8 features of 16 bits, 4 of 32: with 8 of 32 a store's lanes lie 32 bytes apart, 240 us
-// for 63 001 x 2 432 instead of 150).
+// for 63 001 x 2 432 in fp32 instead of 206).  past: from 64 MB on stores go around the caches, which hold the codes then (142 us; 5.4 TB/s).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K, int Kp, int Rp,
-                                                     T* __restrict__ out, long long os)
+                                                     T* __restrict__ out, long long os, int past)
 {
     constexpr int PER = 16 / sizeof(T), LANES = 128 / PER;
     const int c = blockIdx.x * 128 + (threadIdx.x % LANES) * PER, r0 = blockIdx.y * A8_ROWS;
@@ -114,7 +114,11 @@ __global__ void __launch_bounds__(256) k_act8_unpack(const uint8_t* __restrict__
             a8_st(&e[4 * i], a.x * s); a8_st(&e[4 * i + 1], a.y * s); a8_st(&e[4 * i + 2], b.x * s); a8_st(&e[4 * i + 3], b.y * s);
         }
         T* o = out + (long long)r * os + c;
-        if (VEC && K - c >= PER) *(uint4*)o = *(const uint4*)e;
+        typedef unsigned W4 __attribute__((ext_vector_type(4)));
+        if (VEC && K - c >= PER) {
+            if (past) __builtin_nontemporal_store(*(const W4*)e, (W4*)o);
+            else *(W4*)o = *(const W4*)e;
+        }
         else {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
@@ -173,6 +177,7 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
     NF_CHECK_ARG((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "codes and scales must be 16-byte aligned");
     const int es = dtype == 0 ? 4 : 2;
     const bool vec = (uintptr_t)out % 16 == 0 && out_stride * es % 16 == 0;
+    const int past = (long long)rows * K * es >= 64ll << 20;
     const int step = 65535 * A8_ROWS;
     for (int r0 = 0; r0 < rows; r0 += step) {
         const int n = rows - r0 < step ? rows - r0 : step;
@@ -182,9 +187,9 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
     do {                                                                                                                                     \
         T* p = (T*)out + (int64_t)r0 * out_stride;                                                                                           \
         if (vec) hipLaunchKernelGGL((k_act8_unpack<T, true>), grid, dim3(256), 0, (hipStream_t)stream, codes + (size_t)r0 * Kp, scales + r0, n, \
-                                    K, Kp, Rp, p, (long long)out_stride);                                                                    \
+                                    K, Kp, Rp, p, (long long)out_stride, past);                                                                    \
         else hipLaunchKernelGGL((k_act8_unpack<T, false>), grid, dim3(256), 0, (hipStream_t)stream, codes + (size_t)r0 * Kp, scales + r0, n,   \
-                                K, Kp, Rp, p, (long long)out_stride);                                                                        \
+                                K, Kp, Rp, p, (long long)out_stride, past);                                                                        \
     } while (0)
         if (dtype == 0) A8_UNPACK(float);
         else if (dtype == 1) A8_UNPACK(A8Bf16);

@@ -50,6 +50,7 @@ struct NfScanArgs {
     int gate_st, x_st, g_st;             // strides of a step, in bytes (a tile's rows span less than 2^31)
     int B, T, D, nblk, ntiles;
     int gate32, shared, log_gate, reverse;
+    int past;                            // x is too large for the caches: stores go around them
 };
 
 struct NfF32 { typedef float st; static __device__ __forceinline__ float cv(st v) { return v; } static __device__ __forceinline__ st pk(float v) { return v; } };
@@ -157,12 +158,17 @@ template <typename E, int VEC, int TPT, bool SHARED> struct NfGateStretch {
     }
 };
 
-template <typename E, int VEC> __device__ __forceinline__ void nf_put(char* p, const float (&v)[VEC])
+// past: around the caches (uniform), for rows of whole cache lines of a tensor that they would not hold anyway
+template <typename E, int VEC> __device__ __forceinline__ void nf_put(char* p, const float (&v)[VEC], bool past)
 {
     typename NfVec<E, VEC>::type w;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) w[k] = E::pk(v[k]);
-    *(typename NfVec<E, VEC>::type*)p = w;
+    if (past) {          // (between the empty statements: the two stores would be made one, and that an ordinary one)
+        asm volatile("");
+        __builtin_nontemporal_store(w, (typename NfVec<E, VEC>::type*)p);
+        asm volatile("");
+    } else *(typename NfVec<E, VEC>::type*)p = w;
 }
 
 // Which steps of a stretch start / end a sequence and which belong to none (bit i), for packed rows.
@@ -506,6 +512,7 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW, M
     const bool live = ch < a.D;
     const int chl = live ? ch : 0;
     const int T = a.T, rev = a.reverse;
+    const bool past = CG * VEC * ES >= 128 && a.past;
     const int gs = (ES == 4 || a.gate32) ? 4 : 2, hstep = a.D * ES;
     const char* gbase = (const char*)a.gate + b * a.gate_sb;
     const char* xbase = (const char*)a.x + b * a.x_sb;
@@ -603,7 +610,7 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW, M
                 for (int i = 0; i < TPT; ++i) {
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) s[k] = fmaf(A[i][N == 1 ? 0 : k], s[k], x.at(i, k));
-                    nf_put<E, VEC>(hb + ho, s);
+                    nf_put<E, VEC>(hb + ho, s, past);
                     ho += hs;
                 }
             }
@@ -614,8 +621,8 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW, M
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) s[k] = fmaf(A[i][N == 1 ? 0 : k], s[k], x.at(i, k));
                 if (j0 + i < T) {
-                    if (PACKED && (m.none >> i & 1u)) { const float z[VEC] = {}; nf_put<E, VEC>(hb + ho, z); }
-                    else nf_put<E, VEC>(hb + ho, s);
+                    if (PACKED && (m.none >> i & 1u)) { const float z[VEC] = {}; nf_put<E, VEC>(hb + ho, z, past); }
+                    else nf_put<E, VEC>(hb + ho, s, past);
                     if (PACKED ? m.end >> i & 1u : j0 + i == T - 1) {        // the final state is the last step's, to the bit
                         const int q = PACKED ? a.sid[rev ? T - 1 - (j0 + i) : j0 + i] : b;
 #pragma unroll
@@ -646,6 +653,7 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k
     const bool live = ch < a.D;
     const int chl = live ? ch : 0;
     const int T = a.T, rev = a.reverse;
+    const bool past = CG * VEC * ES >= 128 && a.past;
     const int gs = (ES == 4 || a.gate32) ? 4 : 2, hstep = a.D * ES, gstep = a.D * gs;
     const char* gbase = (const char*)a.gate + b * a.gate_sb;
     const char* xbase = (const char*)a.x + b * a.x_sb;
@@ -786,10 +794,10 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k
                     if (SHARED)
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) dsum[i] += dg[k];
-                    if (a.dx) nf_put<E, VEC>(xq + xo, dx);
+                    if (a.dx) nf_put<E, VEC>(xq + xo, dx, past);
                     if (!SHARED && a.dgate) {
-                        if (ES == 4 || a.gate32) nf_put<NfF32, VEC>(gq + go, dg);
-                        else nf_put<E, VEC>(gq + go, dg);
+                        if (ES == 4 || a.gate32) nf_put<NfF32, VEC>(gq + go, dg, past);
+                        else nf_put<E, VEC>(gq + go, dg, past);
                     }
                     if (MARKED && (m.start >> i & 1u) && a.dh0) {
                         const int q = a.sid[rev ? T - 1 - (j0 + i) : j0 + i];

@@ -170,6 +170,9 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     a.nblk = (int)scan_blocks(s);
     a.ntiles = (s->T + tile - 1) / tile;
     a.gate32 = s->gate32 != 0; a.shared = s->shared != 0; a.log_gate = s->log_gate != 0; a.reverse = s->reverse != 0;
+    // From 64 MB a tensor on (a quarter of the last-level cache) what is written would only push out what is still to be read: 8 x 2048 x 2048
+    // bf16 forward 51 us against 62, 4096 x 192 x 32 fp32 backward 48 against 53.  Below, the caller finds h there.
+    a.past = (long long)s->B * s->T * s->D * es >= 64ll << 20;
     if ((long long)a.B * a.nblk * (s->mode == NF_SCAN_CHAIN ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
     const ScanWs ws = scan_workspace(s, backward);
     const size_t n_part = ws.part;
