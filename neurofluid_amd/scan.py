@@ -42,91 +42,105 @@ def _check_state(t, shape, x, what, name):
         raise ValueError(f"{what}: {name} must be float32 {shape} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _describe(gate, x, row_splits, log_gate, reverse):
-    s = _lib.Scan()
-    packed = row_splits is not None
-    s.dtype, s.gate32 = _DTYPES[x.dtype], int(gate.dtype == torch.float32)
-    s.shared, s.log_gate, s.reverse = int(gate.shape[-1] == 1), int(log_gate), int(reverse)
-    s.B, s.T, s.D = (1,) + tuple(x.shape) if packed else tuple(x.shape)
-    s.n_seq = row_splits.numel() - 1 if packed else 0
-    s.row_splits, s.gate, s.x = ptr(row_splits), ptr(gate), ptr(x)
-    s.gate_sb, s.gate_st = (0, gate.stride(0)) if packed else (gate.stride(0), gate.stride(1))
-    s.x_sb, s.x_st = (0, x.stride(0)) if packed else (x.stride(0), x.stride(1))
-    return s
+def _describe(gate, x, row_splits, opts, plan, **p):
+    """nf_scan_t, filled in one go (field by field is slower than the launch)."""
+    log_gate, reverse = opts
+    if row_splits is None:
+        B, T, D = x.shape
+        n_seq, splits = 0, None
+        (gsb, gst, _), (xsb, xst, _) = gate.stride(), x.stride()
+    else:
+        B, (T, D) = 1, x.shape
+        n_seq, splits = row_splits.numel() - 1, row_splits.data_ptr()
+        gsb = xsb = 0
+        gst, xst = gate.stride(0), x.stride(0)
+    get = p.get
+    ysb, yst = get("strides", (0, 0))
+    return _lib.Scan(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[-1] == 1, log_gate, reverse, B, T, D, n_seq, splits, gate.data_ptr(),
+                     x.data_ptr(), get("g"), get("h0"), get("g_last"), gsb, gst, xsb, xst, ysb, yst, get("h"), get("h_last"), get("states"), get("sid"),
+                     get("dgate"), get("dx"), get("dh0"), *plan)
 
 
-def _workspace(lib, s, backward, dev):
-    s.workspace_bytes = lib.nf_scan_workspace_bytes(s, backward)
-    ws = torch.empty(s.workspace_bytes, dtype=torch.uint8, device=dev) if s.workspace_bytes else None
-    s.workspace = ptr(ws)
-    return ws
+def _run(lib, s, backward, x):
+    n = lib.nf_scan_workspace_bytes(s, backward)
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)          # (alive until the launches are enqueued)
+        s.workspace, s.workspace_bytes = ws.data_ptr(), n
+    if backward:
+        check(lib.nf_scan_bwd(s, _lib.raw_stream(x)), "nf_scan_bwd")
+    else:
+        check(lib.nf_scan_fwd(s, _lib.raw_stream(x)), "nf_scan_fwd")
 
 
 @_lib.on_device
-def _forward(x, gate, h0, row_splits, log_gate, reverse, keep):
+def _forward(x, gate, h0, row_splits, opts, keep):
     """-> h, h_last and what the backward needs besides the inputs: (states, sid, plan)."""
     lib = _lib.load()
     dev = x.device
-    s = _describe(gate, x, row_splits, log_gate, reverse)
-    n_state = s.n_seq if row_splits is not None else s.B
+    x, gate = _rows(x), _rows(gate)
+    if h0 is not None:
+        h0 = h0.contiguous()
+    packed = row_splits is not None
+    D = x.shape[-1]
+    n_state = row_splits.numel() - 1 if packed else x.shape[0]
     h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    if s.B == 0 or (s.T == 0 and row_splits is None):
-        last = torch.zeros(n_state, s.D, dtype=torch.float32, device=dev) if h0 is None else h0.clone()
+    if not packed and x.shape[0] * x.shape[1] == 0:
+        last = torch.zeros(n_state, D, dtype=torch.float32, device=dev) if h0 is None else h0.clone()
         return h, last, (None, None, (0, 0, 0))
-    last = torch.empty(n_state, s.D, dtype=torch.float32, device=dev)
+    last = torch.empty((n_state, D), dtype=torch.float32, device=dev)
+    sid = torch.empty(x.shape[0], dtype=torch.int32, device=dev) if packed else None
+    s = _describe(gate, x, row_splits, opts, (0, 0, 0), h=h.data_ptr(), h_last=last.data_ptr(), h0=ptr(h0), sid=ptr(sid))
     n_states = ctypes.c_size_t()
     check(lib.nf_scan_plan(s, n_states), "nf_scan_plan")
-    states = torch.empty(n_states.value, dtype=torch.float32, device=dev) if keep else None
-    sid = torch.empty(s.T, dtype=torch.int32, device=dev) if row_splits is not None else None
-    s.h0, s.h, s.h_last, s.states, s.sid = ptr(h0), h.data_ptr(), last.data_ptr(), ptr(states), ptr(sid)
-    ws = _workspace(lib, s, 0, dev)              # noqa: F841  (alive until the launches are enqueued)
-    check(lib.nf_scan_fwd(s, _lib.raw_stream(x)), "nf_scan_fwd")
+    states = None
+    if keep:
+        states = torch.empty(n_states.value, dtype=torch.float32, device=dev)
+        s.states = states.data_ptr()
+    _run(lib, s, 0, x)
     return h, last, (states, sid, (s.vec, s.cg, s.mode))
 
 
 class _ScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gate, x, h0, row_splits, log_gate, reverse):
+    def forward(ctx, gate, x, h0, row_splits, opts):
         ctx.set_materialize_grads(False)
-        h, last, (states, sid, plan) = _forward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(),
-                                                row_splits, log_gate, reverse, True)
+        h, last, (states, sid, plan) = _forward(x, gate, h0, row_splits, opts, True)
         ctx.save_for_backward(gate, x, h0, row_splits, states, sid)
-        ctx.opts, ctx.plan = (log_gate, reverse), plan
+        ctx.opts, ctx.plan = opts, plan
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, g_last):
         gate, x, h0, row_splits, states, sid = ctx.saved_tensors
-        return _backward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(), row_splits, states, sid, g, g_last,
-                         ctx.opts, ctx.plan, ctx.needs_input_grad) + (None, None, None)
+        return _backward(x, gate, h0, row_splits, states, sid, g, g_last, ctx.opts, ctx.plan, ctx.needs_input_grad) + (None, None)
 
 
 @_lib.on_device
 def _backward(x, gate, h0, row_splits, states, sid, g, g_last, opts, plan, need):
     lib = _lib.load()
     dev = x.device
-    gl = None if g_last is None else g_last.detach().contiguous()
-    s = _describe(gate, x, row_splits, *opts)
-    s.vec, s.cg, s.mode = plan
-    n_state = s.n_seq if row_splits is not None else s.B
+    x, gate = _rows(x), _rows(gate)
+    h0 = None if h0 is None else h0.contiguous()
+    g_last = None if g_last is None else g_last.contiguous()
+    packed = row_splits is not None
+    n_state = row_splits.numel() - 1 if packed else x.shape[0]
     dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[0] else None
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[1] else None
-    dh0 = torch.empty(n_state, s.D, dtype=torch.float32, device=dev) if need[2] else None
-    if s.B == 0 or (s.T == 0 and row_splits is None):
+    dh0 = torch.empty((n_state, x.shape[-1]), dtype=torch.float32, device=dev) if need[2] else None
+    if not packed and x.shape[0] * x.shape[1] == 0:
         if dh0 is not None:
-            dh0.copy_(gl) if gl is not None else dh0.zero_()
+            dh0.copy_(g_last) if g_last is not None else dh0.zero_()
         return dgate, dx, dh0
-    y = None
+    strides = (0, 0)
     if g is not None:
-        y = _rows(g.detach())
-        if y.data_ptr() % (s.vec * y.element_size()) or any(v % s.vec for v in y.stride()[:-1]):
-            y = y.clone(memory_format=torch.contiguous_format)
-        s.g_sb, s.g_st = (0, y.stride(0)) if row_splits is not None else (y.stride(0), y.stride(1))
-    s.g, s.h0, s.g_last, s.states, s.sid = ptr(y), ptr(h0), ptr(gl), ptr(states), ptr(sid)
-    s.dgate, s.dx, s.dh0 = ptr(dgate), ptr(dx), ptr(dh0)
-    ws = _workspace(lib, s, 1, dev)              # noqa: F841
-    check(lib.nf_scan_bwd(s, _lib.raw_stream(x)), "nf_scan_bwd")
+        g, vec = _rows(g), plan[0]
+        if vec > 1 and (g.data_ptr() % (vec * g.element_size()) or any(v % vec for v in g.stride()[:-1])):
+            g = g.clone(memory_format=torch.contiguous_format)
+        strides = (0, g.stride(0)) if packed else g.stride()[:2]
+    s = _describe(gate, x, row_splits, opts, plan, g=ptr(g), strides=strides, g_last=ptr(g_last), h0=ptr(h0), states=ptr(states), sid=ptr(sid),
+                  dgate=ptr(dgate), dx=ptr(dx), dh0=ptr(dh0))
+    _run(lib, s, 1, x)
     return dgate, dx, dh0
 
 
@@ -155,9 +169,10 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     if h0 is not None:
         _check_state(h0, (row_splits.numel() - 1 if packed else x.shape[0], x.shape[-1]), x, what, "h0")
     ops._require_cuda(gate, x)
+    opts = (bool(log_gate), bool(reverse))
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _ScanFn.apply(gate, x, h0, row_splits, bool(log_gate), bool(reverse))
-    return _forward(_rows(x.detach()), _rows(gate.detach()), None if h0 is None else h0.detach().contiguous(), row_splits, log_gate, reverse, False)[:2]
+        return _ScanFn.apply(gate, x, h0, row_splits, opts)
+    return _forward(x, gate, h0, row_splits, opts, False)[:2]
 
 
 def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
