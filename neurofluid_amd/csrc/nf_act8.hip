@@ -239,11 +239,11 @@ template <typename T> struct A8Planes { static constexpr int n = 3; };
 template <> struct A8Planes<A8F16> { static constexpr int n = 2; };
 template <> struct A8Planes<A8Bf16> { static constexpr int n = 1; };
 
-// v = h + (what is returned), h = v with its low 16 bits cleared.  An infinite or NaN v leaves nothing or NaN.
-__device__ __forceinline__ float a8_rest(float v)
+// v = h + (what is returned), h = v with its low 16 bits cleared.  A NaN leaves NaN, an infinity (FIRST: no rest is one) nothing.
+template <bool FIRST> __device__ __forceinline__ float a8_rest(float v)
 {
     const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    return h == v ? 0.f : v - h;
+    return FIRST && h == v ? 0.f : v - h;
 }
 // the upper halves of two words: (low: a, high: b)
 __device__ __forceinline__ unsigned a8_hi2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
             sA[buf][p][wave][64 * c + lane] = make_uint4(a8_hi2(v[0], v[1]), a8_hi2(v[2], v[3]), a8_hi2(v[4], v[5]), a8_hi2(v[6], v[7]));
             if (p + 1 < NP)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = a8_rest(v[i]);
+                for (int i = 0; i < 8; ++i) v[i] = p == 0 ? a8_rest<true>(v[i]) : a8_rest<false>(v[i]);
         } else {
             const int h = (piece - C * NP) / 4, f = (piece - C * NP) % 4;
             if (f < 2) {
