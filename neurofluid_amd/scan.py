@@ -6,12 +6,13 @@ the gate 1 - alpha.  Here channels, gates and direction are the caller's: featur
 over the frames of a sequence.  There is no torch fallback: CPU tensors raise.
 """
 import ctypes
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from ._lib import check, ptr
+from ._lib import check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX_STEPS, _MAX_CHANNELS, _MAX_STRIDE = 1 << 30, 1 << 20, 1 << 18
@@ -42,12 +43,19 @@ def _check_state(t, shape, x, what, name):
         raise ValueError(f"{what}: {name} must be float32 {shape} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+_PACK = struct.Struct("9i4x6P6q7P3i4xPN")          # nf_scan_t's fields, in order
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _describe(gate, x, row_splits, opts, plan, **p):
-    """nf_scan_t, filled in one go (field by field is slower than the launch)."""
+    """nf_scan_t, packed in one go (35 ctypes fields one by one take longer than the launch)."""
     log_gate, reverse = opts
     if row_splits is None:
         B, T, D = x.shape
-        n_seq, splits = 0, None
+        n_seq, splits = 0, 0
         (gsb, gst, _), (xsb, xst, _) = gate.stride(), x.stride()
     else:
         B, (T, D) = 1, x.shape
@@ -56,9 +64,11 @@ def _describe(gate, x, row_splits, opts, plan, **p):
         gst, xst = gate.stride(0), x.stride(0)
     get = p.get
     ysb, yst = get("strides", (0, 0))
-    return _lib.Scan(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[-1] == 1, log_gate, reverse, B, T, D, n_seq, splits, gate.data_ptr(),
-                     x.data_ptr(), get("g"), get("h0"), get("g_last"), gsb, gst, xsb, xst, ysb, yst, get("h"), get("h_last"), get("states"), get("sid"),
-                     get("dgate"), get("dx"), get("dh0"), *plan)
+    buf = bytearray(_PACK.size)
+    _PACK.pack_into(buf, 0, _DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[-1] == 1, log_gate, reverse, B, T, D, n_seq, splits, gate.data_ptr(),
+                    x.data_ptr(), get("g", 0), get("h0", 0), get("g_last", 0), gsb, gst, xsb, xst, ysb, yst, get("h", 0), get("h_last", 0), get("states", 0),
+                    get("sid", 0), get("dgate", 0), get("dx", 0), get("dh0", 0), *plan, 0, 0)
+    return _lib.Scan.from_buffer(buf)
 
 
 def _run(lib, s, backward, x):
@@ -89,7 +99,7 @@ def _forward(x, gate, h0, row_splits, opts, keep):
         return h, last, (None, None, (0, 0, 0))
     last = torch.empty((n_state, D), dtype=torch.float32, device=dev)
     sid = torch.empty(x.shape[0], dtype=torch.int32, device=dev) if packed else None
-    s = _describe(gate, x, row_splits, opts, (0, 0, 0), h=h.data_ptr(), h_last=last.data_ptr(), h0=ptr(h0), sid=ptr(sid))
+    s = _describe(gate, x, row_splits, opts, (0, 0, 0), h=h.data_ptr(), h_last=last.data_ptr(), h0=_ptr(h0), sid=_ptr(sid))
     n_states = ctypes.c_size_t()
     check(lib.nf_scan_plan(s, n_states), "nf_scan_plan")
     states = None
@@ -138,8 +148,8 @@ def _backward(x, gate, h0, row_splits, states, sid, g, g_last, opts, plan, need)
         if vec > 1 and (g.data_ptr() % (vec * g.element_size()) or any(v % vec for v in g.stride()[:-1])):
             g = g.clone(memory_format=torch.contiguous_format)
         strides = (0, g.stride(0)) if packed else g.stride()[:2]
-    s = _describe(gate, x, row_splits, opts, plan, g=ptr(g), strides=strides, g_last=ptr(g_last), h0=ptr(h0), states=ptr(states), sid=ptr(sid),
-                  dgate=ptr(dgate), dx=ptr(dx), dh0=ptr(dh0))
+    s = _describe(gate, x, row_splits, opts, plan, g=_ptr(g), strides=strides, g_last=_ptr(g_last), h0=_ptr(h0), states=_ptr(states), sid=_ptr(sid),
+                  dgate=_ptr(dgate), dx=_ptr(dx), dh0=_ptr(dh0))
     _run(lib, s, 1, x)
     return dgate, dx, dh0
 

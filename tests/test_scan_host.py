@@ -72,3 +72,14 @@ def test_c_entries_refuse():
     # a long, narrow sequence is cut: the plan asks for room for the chunks
     s = _lib.Scan(dtype=1, B=1, T=100000, D=64)
     assert lib.nf_scan_plan(ctypes.byref(s), None) == 0 and lib.nf_scan_workspace_bytes(ctypes.byref(s), 0) > 0
+
+
+def test_the_packed_descriptor_is_the_struct():
+    """scan._PACK writes nf_scan_t as ctypes lays it out (every field with a value of its own)."""
+    from neurofluid_amd import _lib
+    assert scan._PACK.size == ctypes.sizeof(_lib.Scan)
+    names = [n for n, _ in _lib.Scan._fields_]
+    buf = bytearray(scan._PACK.size)
+    scan._PACK.pack_into(buf, 0, *range(1, len(names) + 1))
+    s = _lib.Scan.from_buffer(buf)
+    assert [getattr(s, n) for n in names] == list(range(1, len(names) + 1))
