@@ -46,6 +46,10 @@ class Act8:
         return self.codes.device
 
     @property
+    def tensors(self):
+        return self.codes, self.scales
+
+    @property
     def nbytes(self):
         return self.codes.numel() + self.scales.numel()
 
@@ -146,14 +150,15 @@ class _LinearFn(torch.autograd.Function):
                 y.copy_(bias.detach().expand_as(y))
             if m.shape[0]:
                 ops.gemm(m, w.t(), out=y, accumulate=bias is not None)
-            ctx.ckpt = pack(m) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(weight)
+            ckpt = pack(m) if ctx.needs_input_grad[1] else None
+        ctx.rows = m.shape
+        ctx.save_for_backward(weight, *(ckpt.tensors if ckpt is not None else ()))       # (what is saved goes with the backward, not with ctx)
         return y.view(x.shape[:-1] + (w.shape[0],))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        (weight,) = ctx.saved_tensors
+        weight, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         with torch.cuda.device(g.device):
@@ -164,7 +169,7 @@ class _LinearFn(torch.autograd.Function):
                     ops.gemm(m, weight.detach(), out=dx)
                 dx = dx.view(g.shape[:-1] + (weight.shape[1],))
             if need[1]:
-                dw, db = wgrad(m, ctx.ckpt, bias=need[2])
+                dw, db = wgrad(m, Act8(*kept, ctx.rows, torch.float32), bias=need[2])
             elif need[2]:
                 db = m.sum(0)
         return dx, dw, db

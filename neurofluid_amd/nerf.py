@@ -124,18 +124,20 @@ class _NerfFn(torch.autograd.Function):
             packed_n = ops.pack_nerf_n(packed, cx, cd)
             check(lib.nf_nerf_mlp_fwd_n2(ptr(packed_n), cx, cd, ptr(X), ptr(n_rows), n, ptr(row_sample), ptr(out), ptr(acts), ptr(amask), _lib.stream()),
                   "nf_nerf_mlp_fwd_n2")
-        ctx.act8 = (act8.pack(acts[:n * 2432].view(n, 2432)), act8.pack(xf[:, :cx]), act8.pack(xf[:, cx:]))
+        kept = [act8.pack(acts[:n * 2432].view(n, 2432)), act8.pack(xf[:, :cx]), act8.pack(xf[:, cx:])]
+        ctx.act8 = [(k.shape, k.dtype) for k in kept]
         ctx.net, ctx.sigma_only, ctx.n, ctx.x_needs_grad = net, sigma_only, n, bool(ctx.needs_input_grad[1])
         ctx.save_for_backward(packed, _pack_bwd(net, cx, cd, dev), amask, n_rows, row_sample, out, None,
-                              layers[0].weight.detach().clone(), layers[4].weight.detach().clone(), layers[9].weight.detach().clone())
+                              layers[0].weight.detach().clone(), layers[4].weight.detach().clone(), layers[9].weight.detach().clone(),
+                              *[t for k in kept for t in k.tensors])
         return out[:, 3:4].clone() if sigma_only else out
 
     @staticmethod
-    def _wgrad_act8(ctx, dpre):
+    def _wgrad_act8(ctx, dpre, kept):
         """The 12 weight and 12 bias gradients from the packed activations (first column of dpre, outputs, first feature, features, bias)."""
         from . import act8
         cx, cd = ctx.net.in_channels_xyz, ctx.net.in_channels_dir
-        acts8, xyz8, dir8 = ctx.act8
+        acts8, xyz8, dir8 = [act8.Act8(kept[2 * i], kept[2 * i + 1], *form) for i, form in enumerate(ctx.act8)]
         hidden = [1, 2, 3, 4, 5, 6, 7]
         jobs = [(256 * l, 256, 256 * (l - 1), 256, True) for l in hidden]
         jobs += [(8 * 256, 256, 7 * 256, 256, True), (9 * 256, 128, 8 * 256, 256, True), (2435, 1, 7 * 256, 256, True), (2432, 3, 9 * 256, 128, True)]
@@ -156,7 +158,7 @@ class _NerfFn(torch.autograd.Function):
         net, n = ctx.net, ctx.n
         cx, cd = net.in_channels_xyz, net.in_channels_dir
         layers = net.linear_layers()
-        packed, packed_t, X, n_rows, row_sample, out, acts, W1, W5, Wd = ctx.saved_tensors
+        packed, packed_t, X, n_rows, row_sample, out, acts, W1, W5, Wd, *kept = ctx.saved_tensors
         dev = out.device
         # sigma_only (models/nerf.py:100-113) never touches xyz_encoding_final / dir_encoding / rgb: the reference leaves their
         # .grad at None (an optimiser with weight decay or moment decay must not step them), so do we
@@ -174,7 +176,7 @@ class _NerfFn(torch.autograd.Function):
         if ctx.act8 is not None:         # X holds the mask words here
             check(lib.nf_nerf_mlp_bwd_n2(ptr(packed), ptr(packed_t), cx, cd, ptr(X), ptr(n_rows), n, ptr(row_sample), ptr(out), ptr(d_rs),
                                          ptr(dpre), st), "nf_nerf_mlp_bwd_n2")
-            gw, gb = _NerfFn._wgrad_act8(ctx, dpre)
+            gw, gb = _NerfFn._wgrad_act8(ctx, dpre, kept)
         else:
             check(lib.nf_nerf_mlp_bwd_n(ptr(packed), ptr(packed_t), cx, cd, ptr(acts), ptr(n_rows), n, ptr(row_sample), ptr(out),
                                         ptr(d_rs), ptr(dpre), st), "nf_nerf_mlp_bwd_n")
