@@ -140,20 +140,25 @@ def wgrad(dy, ckpt, bias=True):
     return wgrad_jobs(dy, ckpt, [(0, dy.shape[-1] if dy.dim() else 0, 0, ckpt.features if isinstance(ckpt, Act8) else 0, bias)])[0]
 
 
+@_lib.on_device
+def _linear(x, weight, bias):
+    m, w = _matrix(x.detach()), weight.detach()
+    y = torch.empty(m.shape[0], w.shape[0], dtype=torch.float32, device=x.device)
+    if bias is not None:
+        y.copy_(bias.detach().expand_as(y))
+    if m.shape[0]:
+        ops.gemm(m, w.t(), out=y, accumulate=bias is not None)
+    return y.view(x.shape[:-1] + (w.shape[0],)), m
+
+
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        with torch.cuda.device(x.device):
-            m, w = _matrix(x.detach()), weight.detach()
-            y = torch.empty(m.shape[0], w.shape[0], dtype=torch.float32, device=x.device)
-            if bias is not None:
-                y.copy_(bias.detach().expand_as(y))
-            if m.shape[0]:
-                ops.gemm(m, w.t(), out=y, accumulate=bias is not None)
-            ckpt = pack(m) if ctx.needs_input_grad[1] else None
-        ctx.rows = m.shape
+        y, m = _linear(x, weight, bias)
+        ckpt = pack(m) if ctx.needs_input_grad[1] else None
+        ctx.form = ckpt.shape if ckpt is not None else None
         ctx.save_for_backward(weight, *(ckpt.tensors if ckpt is not None else ()))       # (what is saved goes with the backward, not with ctx)
-        return y.view(x.shape[:-1] + (w.shape[0],))
+        return y
 
     @staticmethod
     @once_differentiable
@@ -169,9 +174,10 @@ class _LinearFn(torch.autograd.Function):
                     ops.gemm(m, weight.detach(), out=dx)
                 dx = dx.view(g.shape[:-1] + (weight.shape[1],))
             if need[1]:
-                dw, db = wgrad(m, Act8(*kept, ctx.rows, torch.float32), bias=need[2])
+                dw, db = wgrad(m, Act8(*kept, ctx.form, torch.float32), bias=need[2])
             elif need[2]:
-                db = m.sum(0)
+                # (a sum by the framework's own product: torch's, over many rows, would leave a memset in a captured graph)
+                db = ops.gemm(torch.ones(1, m.shape[0], device=g.device), m)[0] if m.shape[0] else torch.zeros_like(weight[:, 0])
         return dx, dw, db
 
 
@@ -191,4 +197,6 @@ def linear(x, weight, bias=None):
     if any(t is not None and t.device != x.device for t in (weight, bias)):
         raise ValueError("act8.linear: x, weight and bias are on different devices")
     ops._require_cuda(x)
-    return _LinearFn.apply(x, weight, bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LinearFn.apply(x, weight, bias)
+    return _linear(x, weight, bias)[0]

@@ -230,6 +230,72 @@ def test_linear(dev):
         assert o.shape == lead + (40,) and gz.shape == z.shape and not gw.any()
 
 
+def test_linear_packs_for_a_backward_only(dev, monkeypatch):
+    from neurofluid_amd import act8
+    x, w, b = torch.randn(70, 33, device=dev), torch.randn(5, 33, device=dev, requires_grad=True), torch.randn(5, device=dev, requires_grad=True)
+    want = act8.linear(x, w, b)
+
+    def never(x):
+        raise AssertionError("packed")
+    monkeypatch.setattr(act8, "pack", never)
+    with torch.no_grad():
+        assert torch.equal(act8.linear(x, w, b), want)
+    assert torch.equal(act8.linear(x, w.detach(), b.detach()), want)
+    assert torch.equal(act8.linear(x, w.detach(), b), want)
+
+
+def test_linear_frees_what_it_kept(dev):
+    """A loss that is still held after its backward holds none of the packed inputs."""
+    from neurofluid_amd import act8
+    x, w = torch.randn(20000, 512, device=dev), torch.randn(8, 512, device=dev, requires_grad=True)
+    act8.linear(x, w).sum().backward()
+    before = torch.cuda.memory_allocated()
+    loss = act8.linear(x, w).sum()
+    assert torch.cuda.memory_allocated() - before >= 20000 * 512
+    loss.backward()
+    assert torch.cuda.memory_allocated() - before < 20000 * 512 // 8
+
+
+def test_linear_layouts(dev):
+    """Operands as a model may hold them: expanded rows, a transposed weight, a gradient of one value; the bias alone over many rows, captured."""
+    from neurofluid_amd import act8
+    g = torch.Generator().manual_seed(13)
+    w, b = torch.randn(40, 24, generator=g), torch.randn(40, generator=g)
+    n = (3 * 9000 + 64) * 2.0 ** -23
+    for base, view in ((torch.randn(1, 24, generator=g), lambda t: t.expand(500, 24)), (torch.randn(24, 300, generator=g), lambda t: t.t()),
+                       (torch.randn(500, 1, generator=g), lambda t: t.expand(500, 24)), (torch.randn(9, 7, 30, generator=g), lambda t: t[:, 1:, 2:26])):
+        for turned in (False, True):
+            x, bd = view(base), b.to(dev).requires_grad_()
+            wd = (w.to(dev).t().contiguous().t() if turned else w.to(dev)).requires_grad_()
+            y = act8.linear(view(base.to(dev)), wd, bd)
+            x2 = x.double().reshape(-1, 24)
+            bound = 32 * 2.0 ** -23 * (x2.abs() @ w.double().abs().t() + b.double().abs())
+            assert ((y.detach().cpu().double().reshape(-1, 40) - (x2 @ w.double().t() + b.double())).abs() <= bound).all()
+            y.sum().backward()          # the gradient comes as one expanded value
+            q = quantised(x.reshape(-1, 24).contiguous())
+            assert ((wd.grad.cpu().double() - q.sum(0).expand(40, 24)).abs() <= n * q.abs().sum(0)).all()
+            assert torch.equal(bd.grad.cpu(), torch.full((40,), float(x2.shape[0])))
+    one = [torch.full(k, v, device=dev, requires_grad=True) for k, v in (((3, 1), 2.0), ((1, 1), 5.0), ((1,), 0.25))]
+    act8.linear(*one).sum().backward()
+    assert [float(t.grad.sum()) for t in one] == [15.0, 6.0, 3.0]
+    x, gy = torch.randn(9000, 24, generator=g).to(dev), torch.randn(9000, 40, generator=g).to(dev)
+    leaf = b.to(dev).requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(act8.linear(x, w.to(dev), leaf), leaf, gy)
+    torch.cuda.current_stream().wait_stream(side)
+    wd, gr = w.to(dev), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        db, = torch.autograd.grad(act8.linear(x, wd, leaf), leaf, gy)
+    for it in range(4):
+        gy.mul_(-1.5)
+        gr.replay()
+        torch.cuda.synchronize()
+        g2 = gy.cpu().double()
+        assert ((db.cpu().double() - g2.sum(0)).abs() <= n * g2.abs().sum(0)).all()
+
+
 def test_streams_and_graphs(dev):
     from neurofluid_amd import act8
     g = torch.Generator().manual_seed(11)
