@@ -45,6 +45,13 @@ class Act8:
     def device(self):
         return self.codes.device
 
+    def _whole(self, what):
+        """The kernels read what the shape says: refuse less."""
+        rows, blocks = self.rows, (self.features + 31) // 32
+        for t, n, name in ((self.codes, 32 * rows * blocks, "codes"), (self.scales, (rows + 63) // 64 * 64 * blocks, "scales")):
+            if t.dtype is not torch.uint8 or t.numel() < n or not t.is_contiguous() or t.device != self.codes.device:
+                raise ValueError(f"{what}: {name} of {self.shape} must be {n} adjacent bytes on one device, got {t.dtype} {tuple(t.shape)}")
+
     @property
     def tensors(self):
         return self.codes, self.scales
@@ -58,6 +65,7 @@ class Act8:
         dtype = dtype or self.dtype
         if dtype not in _DTYPES:
             raise TypeError(f"Act8.unpack: float32, bfloat16 or float16, not {dtype}")
+        self._whole("Act8.unpack")
         return _unpack(self.codes, self, dtype)
 
 
@@ -103,6 +111,8 @@ def wgrad_jobs(dy, ckpt, jobs):
         raise TypeError(f"act8.wgrad: dy must be float32, bfloat16 or float16, not {dy.dtype}")
     if not isinstance(ckpt, Act8):
         raise TypeError("act8.wgrad: the activations must be an Act8 (act8.pack)")
+    if any(abs(int(v)) > _MAX for job in jobs for v in job[:4]):
+        raise ValueError(f"act8.wgrad: a job's numbers pass {_MAX}")
     if dy.dim() < 1 or dy.shape[-1] < 1 or ckpt.features < 1 or dy.numel() // dy.shape[-1] != ckpt.rows:
         raise ValueError(f"act8.wgrad: dy {tuple(dy.shape)} does not fit activations {ckpt.shape}")
     if not 1 <= len(jobs) <= 16:
@@ -110,6 +120,7 @@ def wgrad_jobs(dy, ckpt, jobs):
     ops._require_cuda(dy)
     if dy.device != ckpt.device:
         raise ValueError("act8.wgrad: dy and the activations are on different devices")
+    ckpt._whole("act8.wgrad")
     return _wgrad(dy, ckpt, jobs)
 
 

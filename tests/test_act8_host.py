@@ -30,6 +30,21 @@ def test_wgrad_refuses(dy, ck, err):
         act8.wgrad(dy, ck)
 
 
+def test_wgrad_refuses_numbers_that_the_c_entry_would_cut():
+    for job in ((0, 2 ** 32 + 5, 0, 6, True), (2 ** 32, 5, 0, 6, True), (0, 5, 0, 2 ** 33 + 6, False)):
+        with pytest.raises(ValueError, match="pass"):
+            act8.wgrad_jobs(t(4, 5), fake(4, 6), [job])
+
+
+def test_a_checkpoint_that_is_not_whole_is_refused():
+    whole = fake(70, 40)
+    for codes, scales in ((whole.codes[:-1], whole.scales), (whole.codes, t(255, dtype=torch.uint8)), (whole.codes, t(256)),
+                          (t(2 * whole.codes.numel(), dtype=torch.uint8)[::2], t(256, dtype=torch.uint8))):
+        with pytest.raises(ValueError, match="must be"):
+            act8.Act8(codes, scales, (70, 40), torch.float32).unpack()
+    act8.Act8(whole.codes, t(256, dtype=torch.uint8), (70, 40), torch.float32)._whole("here")
+
+
 def test_unpack_refuses():
     with pytest.raises(TypeError):
         fake(2, 3).unpack(torch.float64)
@@ -67,6 +82,10 @@ def test_c_entries_refuse():
     for bad in (job(0, 5, 0, 4, 1), job(1, 4, 0, 4, 1), job(0, 4, 16, 4, 1), job(0, 4, 0, 65, 1), job(-1, 2, 0, 4, 1), job(0, 0, 0, 4, 1), job(2 ** 31 - 1, 2, 0, 4, 1)):
         assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 1, bad, None, None, None, None) < 0
         assert lib.nf_act8_wgrad_workspace_floats(8, 4, 64, 1, bad) == 0
+    for dy_cols, x_cols in ((2 ** 31 - 1, 64), (4, 2 ** 31 - 1)):
+        assert lib.nf_act8_wgrad(0, None, 4, dy_cols, None, None, x_cols, 8, 1, job(0, 4, 0, 4, 1), None, None, None, None) < 0 and b"bad sizes" in lib.nf_last_error()
+    many = (_lib.Act8Job * 2)(_lib.Act8Job(0, 2 ** 30, 0, 1, 1), _lib.Act8Job(0, 2 ** 30, 0, 1, 1))
+    assert lib.nf_act8_wgrad(0, None, 4, 2 ** 30, None, None, 64, 8, 2, many, None, None, None, None) < 0 and b"outputs" in lib.nf_last_error()
     ok = job(0, 4, 32, 4, 1)
     assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 0, ok, None, None, None, None) < 0
     assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 1, ok, None, None, None, None) < 0 and b"null" in lib.nf_last_error()
