@@ -112,19 +112,35 @@ def test_nerf_trains_on_packed_activations(dev):
 def test_nerf_keeps_less(dev):
     from neurofluid_amd.nerf import NeRF
     kept = []
+
+    def requested():         # (what memory_allocated counts depends on the free blocks that earlier tests left: up to 1 MB more a tensor)
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
     for ck in (None, "e4m3"):
         net = NeRF(in_channels_xyz=198, in_channels_dir=54, act_checkpoint=ck).to(dev)
         x = torch.randn(40000, 252, device=dev)
         out = net(x[:64])
         del out
         torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        before = requested()
         out = net(x)
-        kept.append((torch.cuda.memory_allocated() - before) / 40000)
+        kept.append((requested() - before) / 40000)
         del out
     # 2432 + 252 floats a row, against codes and scales of 2432 + 224 + 64 features (2 805 B), ten mask words of four waves x 64 lanes a
     # 32-row tile (320 B), output and index (20 B); either way two weight blobs of 0.67 M floats and three weights of 0.21 M: 155 B a row of 40 000
     assert kept[0] > 4 * (2432 + 252) and kept[1] < 2805 + 320 + 20 + 160 + 20, kept
+
+
+def test_nerf_frees_what_it_kept(dev):
+    """A loss that is still held after its backward holds none of the packed activations."""
+    from neurofluid_amd.nerf import NeRF
+    net = NeRF(in_channels_xyz=198, in_channels_dir=54, act_checkpoint="e4m3").to(dev)
+    x = torch.randn(20000, 252, device=dev)
+    net(x).sum().backward()
+    before = torch.cuda.memory_allocated()
+    loss = net(x).sum()
+    assert torch.cuda.memory_allocated() - before >= 20000 * 2432
+    loss.backward()
+    assert torch.cuda.memory_allocated() - before < 20000 * 2432 // 4
 
 
 def test_feature_field_along_rays(dev):
