@@ -592,7 +592,7 @@ int nf_trans_step(const nf_trans_step_t* s /*[host]*/, const float* pos, const f
  * step by step.  Results repeat bit for bit.
  * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, mode; *state_floats = the size
  * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_bytes =
- * nf_scan_workspace_bytes(s, backward) bytes, 8-byte aligned, for this call alone.  T <= 2^30, D <= 2^20, step strides < 2^19 elements or so (a tile's rows span less than 2^31 bytes).  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
+ * nf_scan_workspace_bytes(s, backward) bytes, 8-byte aligned, for this call alone.  T <= 2^30, D <= 2^20, step strides < 2^18 elements (a tile's rows span less than 2^32 bytes).  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,
  * h0, states (and sid).
  * row_splits (device, n_seq + 1, ascending): B = 1 and the T rows hold n_seq sequences behind one another, h0 / h_last / g_last / dh0 have
  * one row for each (an empty sequence passes them through); h, dx, dgate are zero on rows that belong to none.  sid: T ints, filled by the

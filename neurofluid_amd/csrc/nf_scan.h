@@ -47,9 +47,10 @@ struct NfScanArgs {
     unsigned long long* ws_tile; unsigned long long* ws_group; unsigned long long* ws_set;      // [k][chain][CG * VEC]
     int* ticket;
     long long gate_sb, x_sb, g_sb;       // strides of a batch, in bytes
-    int gate_st, x_st, g_st;             // strides of a step, in bytes (a tile's rows span less than 2^31)
+    int gate_st, x_st, g_st;             // strides of a step, in bytes (a tile's rows span less than 2^32)
     int B, T, D, nblk, ntiles;
     int gate32, shared, log_gate, reverse;
+    int chain0;                          // NF_SCAN_WAVE: the launch's first chain
     int past;                            // x is too large for the caches: stores go around them
 };
 
@@ -480,7 +481,7 @@ template <int MODE> __device__ __forceinline__ NfPlace nf_place(const NfScanArgs
         p.k = 0;
         p.w = wave;
     } else {
-        p.chain = blockIdx.x * (NF_SCAN_WG / 64) + wave;
+        p.chain = a.chain0 + blockIdx.x * (NF_SCAN_WG / 64) + wave;
         p.k = p.w = 0;
     }
     p.ok = p.chain < nchains;
@@ -852,9 +853,12 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k
 // step: 65 536 steps x 256 channels, fp32, chained forward 46 us against 76; fp16 41 against 63).
 #define NF_SCAN_TPT(vec, mode) (((vec) == 4 ? 4 : 8) * ((mode) == NF_SCAN_WAVE ? 1 : 2))
 #define NF_SCAN_NW(mode) ((mode) == NF_SCAN_WAVE ? 1 : 8)
+// (a launch has fewer than 2^32 threads: more chains than NF_SCAN_SLICE by waves take several launches, the other modes are refused)
+#define NF_SCAN_SLICE (1 << 25)
+#define NF_SCAN_MAX_TILES ((1 << 23) - 1)
 template <typename E> int nf_scan_launch(const NfScanArgs& a, int vec, int cg, int mode, int backward, hipStream_t st)
 {
-    const long long chains = (long long)a.B * a.nblk;
+    const long long all = (long long)a.B * a.nblk, chains = mode == NF_SCAN_WAVE && all - a.chain0 > NF_SCAN_SLICE ? NF_SCAN_SLICE : all - a.chain0;
     const dim3 grid((unsigned)(mode == NF_SCAN_WAVE ? (chains + NF_SCAN_WG / 64 - 1) / (NF_SCAN_WG / 64) : mode == NF_SCAN_WALK ? chains : chains * a.ntiles));
     const int packed = a.sid != nullptr;
 #define NF_SCAN_GO(V, C, M, PK, SH)                                                                                                                          \

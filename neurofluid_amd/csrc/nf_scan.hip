@@ -98,11 +98,11 @@ __global__ void __launch_bounds__(256) k_scan_rows(const int64_t* __restrict__ r
 __global__ void __launch_bounds__(256) k_scan_empty(const int64_t* __restrict__ rs, int n_seq, int T, int D, const float* __restrict__ src,
                                                     float* __restrict__ dst)
 {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= (long long)n_seq * D) return;
-    const int s = (int)(e / D);
-    const int64_t a = min(max(rs[s], (int64_t)0), (int64_t)T), b = min(max(rs[s + 1], (int64_t)0), (int64_t)T);
-    if (a >= b) dst[e] = src ? src[e] : 0.f;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < (long long)n_seq * D; e += (long long)gridDim.x * 256) {
+        const int s = (int)(e / D);
+        const int64_t a = min(max(rs[s], (int64_t)0), (int64_t)T), b = min(max(rs[s + 1], (int64_t)0), (int64_t)T);
+        if (a >= b) dst[e] = src ? src[e] : 0.f;
+    }
 }
 
 // The chain's entries are set to "empty", the counters of tiles to 0 (a kernel: a memset node in a captured graph has given wrong results).
@@ -140,8 +140,8 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     float* fin = backward ? s->dh0 : s->h_last;
     if (!backward && !fin && n_state > 0) { nf_set_error("%s: null h_last", who); return NF_EINVAL; }
     if (packed && s->n_seq > 0 && fin) {
-        const long long n = (long long)s->n_seq * s->D;
-        hipLaunchKernelGGL(k_scan_empty, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->D, init, fin);
+        const long long blocks = ((long long)s->n_seq * s->D + 255) / 256;
+        hipLaunchKernelGGL(k_scan_empty, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->D, init, fin);
         NF_CHECK_LAUNCH();
     }
     if (s->B == 0 || s->T == 0) return NF_OK;        // (dense with T = 0: the caller copies the state)
@@ -158,9 +158,10 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     a.gate = s->gate; a.x = s->x; a.g = s->g; a.h0 = s->h0; a.g_last = s->g_last; a.h = s->h; a.h_last = s->h_last; a.states = s->states;
     a.dgate = s->dgate; a.dx = s->dx; a.dh0 = s->dh0; a.sid = packed ? s->sid : nullptr;
     const int tile = scan_tile(s);
-    const int64_t far = 0x7fffffff / tile / 4;
+    const int64_t far = 0xffffffffll / tile / 4;         // (a tile's rows: unsigned 32-bit offsets)
     const int64_t gate_st = s->T > 1 ? s->gate_st : 0, x_st = s->T > 1 ? s->x_st : 0, g_st = s->T > 1 ? s->g_st : 0;
-    if (gate_st < 0 || x_st < 0 || g_st < 0 || gate_st > far || x_st > far || g_st > far) {
+    if (gate_st < 0 || x_st < 0 || g_st < 0 || gate_st > far || x_st > far || g_st > far ||
+        (s->T > 1 && s->D > far)) {
         nf_set_error("%s: steps of a tensor lie too far apart (copy it)", who);
         return NF_EINVAL;
     }
@@ -173,7 +174,8 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     // From 64 MB a tensor on (a quarter of the last-level cache) what is written would only push out what is still to be read: 8 x 2048 x 2048
     // bf16 forward 51 us against 62, 4096 x 192 x 32 fp32 backward 48 against 53.  Below, the caller finds h there.
     a.past = (long long)s->B * s->T * s->D * es >= 64ll << 20;
-    if ((long long)a.B * a.nblk * (s->mode == NF_SCAN_CHAIN ? a.ntiles : 1) > 0x7fffffffLL) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
+    const long long chains = (long long)a.B * a.nblk;
+    if (chains > 0x7ffffff0LL || (s->mode != NF_SCAN_WAVE && chains * (s->mode == NF_SCAN_CHAIN ? a.ntiles : 1) > NF_SCAN_MAX_TILES)) { nf_set_error("%s: too many chains", who); return NF_EINVAL; }
     const ScanWs ws = scan_workspace(s, backward);
     const size_t n_part = ws.part;
     if (s->workspace_bytes < 8 * ws.words() || (ws.words() && (!s->workspace || (uintptr_t)s->workspace % 8))) {
@@ -192,8 +194,11 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
         hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, words, ws.entries(), n);
         NF_CHECK_LAUNCH();
     }
-    if (!scan_go(s, a, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
-    NF_CHECK_LAUNCH();
+    for (long long c = 0; c < chains; c += s->mode == NF_SCAN_WAVE ? NF_SCAN_SLICE : chains) {
+        a.chain0 = (int)c;
+        if (!scan_go(s, a, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
+        NF_CHECK_LAUNCH();
+    }
     if (n_part) {
         const long long n = (long long)s->B * s->T;
         hipLaunchKernelGGL(k_scan_fold, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (const float*)a.dgate_part, a.nblk, n,
@@ -269,7 +274,7 @@ extern "C" int nf_scan_step(int dtype, int gate32, int shared, int log_gate, int
                     (uintptr_t)next % 16 == 0 && next_stride % 4 == 0 && (uintptr_t)h % (4 * es) == 0 &&
                     (shared || ((uintptr_t)gate % (4 * gs) == 0 && gate_stride % 4 == 0));
     const long long threads = a.n / (v4 ? 4 : 1);
-    NF_CHECK_ARG((threads + 255) / 256 <= 0x7fffffffLL, "too many elements");
+    NF_CHECK_ARG(threads <= 0xffffff00LL, "too many elements");         // (a launch has fewer than 2^32 threads)
     const dim3 grid((unsigned)((threads + 255) / 256));
     hipStream_t st = (hipStream_t)stream;
 #define NF_STEP(E)                                                                                     \

@@ -15,7 +15,7 @@ from . import _lib, ops
 from ._lib import check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_MAX_STEPS, _MAX_CHANNELS, _MAX_STRIDE = 1 << 30, 1 << 20, 1 << 18
+_MAX_STEPS, _MAX_CHANNELS, _MAX_STRIDE = 1 << 30, 1 << 20, 1 << 17
 
 
 def _rows(t):

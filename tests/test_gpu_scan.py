@@ -279,6 +279,63 @@ def test_long_offsets(dev):
     assert (last[-1] - last1[0]).abs().max() <= 2 * e
 
 
+def test_far_apart_and_widest_rows(dev):
+    """The widest rows that are taken, packed (a tile's rows span 2 GiB), and steps that lie as far apart as a view may have them."""
+    from neurofluid_amd import scan
+    D, cuts = 1 << 20, (0, 1, 4)
+    g = torch.Generator(device=dev).manual_seed(3)
+    gate, x = torch.rand(4, D, device=dev, generator=g), torch.randn(4, D, device=dev, generator=g)
+    rs = torch.tensor(cuts, device=dev)
+    for reverse in (False, True):
+        gd, xd = gate.clone().requires_grad_(), x.clone().requires_grad_()
+        h, last = scan.gated_scan(gd, xd, row_splits=rs, reverse=reverse)
+        h.sum().backward()
+        want, dx = torch.empty_like(x, dtype=torch.float64), torch.empty_like(x, dtype=torch.float64)
+        for a, b in zip(cuts, cuts[1:]):
+            order = list(range(a, b))[::-1] if reverse else list(range(a, b))
+            s = torch.zeros(D, dtype=torch.float64, device=dev)
+            for j in order:
+                s = gate[j].double() * s + x[j].double()
+                want[j] = s
+            u = torch.zeros_like(s)
+            for j in order[::-1]:
+                dx[j] = 1 + u
+                u = gate[j].double() * dx[j]
+        # at most three steps: a rounding each of the product, the sum and the carry, of sums below 3 max |x|
+        assert (h.detach().double() - want).abs().max() <= 9 * 2.0 ** -24 * 3 * float(x.abs().max())
+        assert (xd.grad.double() - dx).abs().max() <= 9 * 2.0 ** -24 * 3
+    T, far = 8300, 150000          # two channels of rows that are 150 000 wide; more than two tiles of 4 096 steps
+    for width in (far, 1 << 17, (1 << 17) + 1):
+        wide = torch.zeros(T, width, dtype=torch.bfloat16, device=dev)
+        wide[:, 1:3] = torch.randn(T, 2, device=dev, generator=g).bfloat16()
+        gt = torch.rand(1, T, 1, device=dev, generator=g)
+        view = wide[None, :, 1:3]
+        a, b = scan.gated_scan(gt, view), scan.gated_scan(gt, view.contiguous())
+        s = torch.zeros(2, dtype=torch.float64)
+        gc, xc, want = gt.cpu().double().view(-1), view[0].cpu().double(), []
+        for t in range(T):
+            s = gc[t] * s + xc[t]
+            want.append(s)
+        want = torch.stack(want)
+        # gates below one, uniform: what is kept is the sum of a few values; 64 fp32 roundings of the largest and bf16's half step
+        tol = 64 * 2.0 ** -24 * want.abs().max() + want.abs() * 2.0 ** -8
+        assert ((a[0][0].cpu().double() - want).abs() <= tol).all() and ((b[0][0].cpu().double() - want).abs() <= tol).all()
+        del wide, view
+
+
+def test_more_chains_than_a_launch_takes(dev):
+    from neurofluid_amd import scan
+    B = (1 << 26) + 5
+    x, gate = torch.ones(B, 1, 1, dtype=torch.bfloat16, device=dev), torch.full((B, 1, 1), 0.5, dtype=torch.bfloat16, device=dev)
+    h0 = torch.full((B, 1), 4.0, device=dev)
+    h0[-1] = 8.0
+    xr = x.requires_grad_()
+    h, last = scan.gated_scan(gate, xr, h0)
+    assert float(last[-1]) == 5.0 and bool((last[:-1] == 3.0).all()) and float(h[-1]) == 5.0 and bool((h[:-1] == 3.0).all())
+    dx, = torch.autograd.grad(h, xr, gate)
+    assert bool((dx == 0.5).all())
+
+
 def test_differences(dev):
     """Directional derivative by central differences; f = <w, h> + <v, h_last> is linear in x and h0, smooth in the gate."""
     from neurofluid_amd import scan
