@@ -28,6 +28,8 @@ def _rows(t):
 def _check(gate, x, what):
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what}: x must be float32, bfloat16 or float16, not {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"{what}: x needs an axis of steps or rows and one of channels, got {tuple(x.shape)}")
     if gate.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"{what}: the gate must have x's dtype or float32, not {gate.dtype}")
     if gate.shape != x.shape and (gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] != 1):
@@ -164,7 +166,7 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     rows that belong to no sequence.
 
     Sums, states and the carries between stretches are float32; h is rounded once.  Gates are meant to be decays, |A| <= 1: products of larger ones over long
-    stretches overflow.  Differentiable once in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
+    stretches overflow, and where a product of gates has reached zero an infinite state goes on as NaN.  Differentiable once in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
     what = "gated_scan"
     _check(gate, x, what)
     packed = row_splits is not None
@@ -188,7 +190,7 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
 def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
     """One step for every row: the new state A * state + x goes to ``out`` (by default into ``state`` itself), its value in x's dtype is returned.
 
-    x: (rows, D); gate: x's shape or (rows, 1); state, out: (rows, D) float32 with adjacent channels.  For inference: no gradients."""
+    x: (rows, D); gate: x's shape or (rows, 1); state, out: (rows, D) float32 with adjacent channels.  x and gate may lie in the same memory.  For inference: no gradients."""
     what = "gated_scan_step"
     _check(gate, x, what)
     if x.dim() != 2:
@@ -212,8 +214,17 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
 
 @_lib.on_device
 def _step(x, gate, state, state_stride, out, out_stride, log_gate):
-    g_, x_ = _rows(gate), _rows(x)
     rows, D = x.shape
+    lo, hi = out, out + 4 * ((rows - 1) * out_stride + D)
+
+    def source(t):           # a copy of what lies among the states that are written, unless it is them, element for element
+        t = _rows(t)
+        p, s = t.data_ptr(), t.stride(0)
+        if p < hi and lo < p + t.element_size() * ((rows - 1) * s + t.shape[1]):
+            if p != out or s != out_stride or t.shape[1] != D or t.dtype is not torch.float32:
+                return t.clone(memory_format=torch.contiguous_format)
+        return t
+    g_, x_ = source(gate), source(x)
     h = torch.empty((rows, D), dtype=x.dtype, device=x.device)
     if rows:
         check(_lib.load().nf_scan_step(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[1] == 1, bool(log_gate), rows, D, g_.data_ptr(),

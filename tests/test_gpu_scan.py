@@ -331,7 +331,8 @@ def test_more_chains_than_a_launch_takes(dev):
     h0[-1] = 8.0
     xr = x.requires_grad_()
     h, last = scan.gated_scan(gate, xr, h0)
-    assert float(last[-1]) == 5.0 and bool((last[:-1] == 3.0).all()) and float(h[-1]) == 5.0 and bool((h[:-1] == 3.0).all())
+    hd, ld = h.detach(), last.detach()
+    assert float(ld[-1]) == 5.0 and bool((ld[:-1] == 3.0).all()) and float(hd[-1]) == 5.0 and bool((hd[:-1] == 3.0).all())
     dx, = torch.autograd.grad(h, xr, gate)
     assert bool((dx == 0.5).all())
 
@@ -434,6 +435,54 @@ def test_step(dev, rows, D, dtype, gate_kind, log_gate):
     assert torch.equal(state.cpu(), s0) and (out[:, D:] == 7).all()
     h2 = scan.gated_scan_step(gate.to(dev), x.to(dev), state, log_gate=log_gate)
     assert torch.equal(h2, h) and torch.equal(state, out[:, :D])
+
+
+def test_step_reads_what_it_overwrites(dev):
+    """Inputs that lie among the states that are written: the gates a column of theirs, x the states themselves, shifted, or between them."""
+    from neurofluid_amd import scan
+    g = torch.Generator().manual_seed(21)
+    base = torch.rand(300, 3 * 64 + 8, generator=g)
+
+    def views(b):
+        s = b[:, :64]
+        yield s, b[:, 8:9], b[:, 70:134]              # one gate a row, from the state's own row
+        yield s, b[:, 64:128], s                      # x is the state
+        yield s, s, s
+        yield s, b[:, 4:68], b[:, 1:65]               # shifted
+        yield s, b[:, 64:128], b[:, 128:192]          # in the same rows, beside it
+        yield b[1:, :64], b[:-1, :64], b[:-1, 64:128]       # a row later
+    for k in range(6):
+        want = [t.double() for t in list(views(base))[k]]
+        want = want[1] * want[0] + want[2]
+        state, gate, x = list(views(base.to(dev)))[k]
+        keep = state.clone()
+        h = scan.gated_scan_step(gate, x, state)
+        assert torch.equal(h, state) and not torch.equal(state, keep)
+        assert ((h.cpu().double() - want).abs() <= 2.0 ** -23 * want.abs()).all(), k
+
+
+def test_two_at_once(dev):
+    """Chained scans that wait for one another's tiles, on two streams together and with one thread's gradients beside another's."""
+    from neurofluid_amd import scan
+    g = torch.Generator().manual_seed(22)
+    data = [(torch.rand(1, 40000, 96, generator=g).to(dev), torch.randn(1, 40000, 96, generator=g).to(dev)) for _ in range(2)]
+
+    def work(gate, x):
+        gate, x = gate.clone().requires_grad_(), x.clone().requires_grad_()
+        h, _ = scan.gated_scan(gate, x)
+        return (h,) + torch.autograd.grad(h, [gate, x], x.detach())
+    want = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = [[], []]
+    for _ in range(6):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(work(*data[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
 
 
 def test_steps_make_a_scan(dev):

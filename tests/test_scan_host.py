@@ -48,6 +48,15 @@ def test_gated_scan_step_refuses(gate, x, state, kw, err):
         scan.gated_scan_step(gate, x, state, **kw)
 
 
+def test_no_axis_of_steps_is_refused():
+    one = torch.ones(5)
+    for x in (one, one[0]):
+        with pytest.raises(ValueError, match="axis"):
+            scan.gated_scan(x, x)
+        with pytest.raises(ValueError, match="axis"):
+            scan.gated_scan_step(x, x, x)
+
+
 def test_gated_scan_step_refuses_an_out_that_overlaps_the_state():
     buf = t(6, 3)
     with pytest.raises(ValueError, match="overlaps"):
