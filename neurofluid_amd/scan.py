@@ -212,22 +212,30 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
     return _step(x, gate, a, sa, b, sb, log_gate)
 
 
+def _apart(t, out, out_stride, rows, D):
+    """A copy of an input that lies among the states that are written, unless it is them, element for element."""
+    p, s = t.data_ptr(), t.stride(0)
+    if p >= out + 4 * ((rows - 1) * out_stride + D) or out >= p + t.element_size() * ((rows - 1) * s + t.shape[1]):
+        return t
+    if p == out and t.shape[1] == D and t.dtype is torch.float32 and (s == out_stride or rows == 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 @_lib.on_device
 def _step(x, gate, state, state_stride, out, out_stride, log_gate):
     rows, D = x.shape
-    lo, hi = out, out + 4 * ((rows - 1) * out_stride + D)
-
-    def source(t):           # a copy of what lies among the states that are written, unless it is them, element for element
-        t = _rows(t)
-        p, s = t.data_ptr(), t.stride(0)
-        if p < hi and lo < p + t.element_size() * ((rows - 1) * s + t.shape[1]):
-            if p != out or s != out_stride or t.shape[1] != D or t.dtype is not torch.float32:
-                return t.clone(memory_format=torch.contiguous_format)
-        return t
-    g_, x_ = source(gate), source(x)
+    g_, x_ = _rows(gate), _rows(x)
+    gp, gs, xp, xs = g_.data_ptr(), g_.stride(0), x_.data_ptr(), x_.stride(0)
+    end = out + 4 * (rows * out_stride + D)            # (generous bounds; _apart looks closer)
+    if gp < end and out < gp + 4 * (rows * gs + D):
+        g_ = _apart(g_, out, out_stride, rows, D)
+        gp, gs = g_.data_ptr(), g_.stride(0)
+    if xp < end and out < xp + 4 * (rows * xs + D):
+        x_ = _apart(x_, out, out_stride, rows, D)
+        xp, xs = x_.data_ptr(), x_.stride(0)
     h = torch.empty((rows, D), dtype=x.dtype, device=x.device)
     if rows:
-        check(_lib.load().nf_scan_step(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[1] == 1, bool(log_gate), rows, D, g_.data_ptr(),
-                                       g_.stride(0), x_.data_ptr(), x_.stride(0), state, state_stride, out, out_stride, h.data_ptr(),
-                                       _lib.raw_stream(x)), "nf_scan_step")
+        check(_lib.load().nf_scan_step(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[1] == 1, bool(log_gate), rows, D, gp, gs, xp, xs,
+                                       state, state_stride, out, out_stride, h.data_ptr(), _lib.raw_stream(x)), "nf_scan_step")
     return h
