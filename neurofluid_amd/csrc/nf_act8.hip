@@ -1,7 +1,8 @@
 // nf_act8.hip — activations kept in 8 bits between forward and backward, and the weight gradient that reads them.
 //
 // Form: e4m3 codes with one power-of-two scale for every 32 features of a row.  2^k is the smallest power that brings the block's largest finite
-// magnitude to 448 (e4m3's largest) or less, k >= -110; code = x / 2^k rounded to nearest even (the division is exact).  So nothing saturates (but magnitudes above 1.875 2^127), a
+// magnitude to 448 (e4m3's largest) or less, k >= -110; code = x / 2^k rounded to nearest even (the division is exact).  So nothing saturates (but magnitudes above
+// 1.875 2^127), a
 // value is off by at most 2^-4 of itself or 2^-10 2^k, and whatever is not finite becomes NaN, in its own place only.  Codes are rows of
 // Kp = 32 ceil(K / 32) bytes (zeros behind K); scales (k + 127, a byte) lie block by block, [Kp / 32][64 ceil(rows / 64)], so that the reader of
 // a column of blocks finds eight rows' scales in eight adjacent bytes.
@@ -24,7 +25,8 @@ __device__ __forceinline__ void a8_st(A8Bf16* p, float v) { p->u = __builtin_bit
 __device__ __forceinline__ void a8_st(A8F16* p, float v) { p->u = __builtin_bit_cast(unsigned short, (_Float16)v); }
 
 // ------------------------------------------------------------------------------------------------
-// pack / unpack: a thread holds 8 adjacent features, four neighbours a block; a workgroup 64 rows x 128 features.
+// pack / unpack: a thread holds 8 adjacent features, four neighbours a block; a workgroup 64 rows x 128 features.  One pass, bound by memory:
+// 63 001 x 2 432 fp32, 613 MB in and 158 MB out, 171 us (4.5 TB/s), and 133 us back (5.8 TB/s: the codes are still in the caches).
 // ------------------------------------------------------------------------------------------------
 template <typename T, bool VEC> __device__ __forceinline__ void a8_load8(const T* p, int left, float (&v)[8])
 {
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(256) k_act8_pack(const T* __restrict__ x, long
 }
 
 // A thread writes 16 bytes, next to its neighbours' (8 features of 16 bits, 4 of 32: with 8 of 32 a store's lanes lie 32 bytes apart, 240 us
-// for 63 001 x 2 432 in fp32 instead of 206).  past: from 64 MB on stores go around the caches, which hold the codes then (142 us; 5.4 TB/s).
+// for 63 001 x 2 432 in fp32 instead of 206).  past: from 64 MB on stores go around the caches, which hold the codes then (133 us).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K, int Kp, int Rp,
                                                      T* __restrict__ out, long long os, int past)
@@ -204,9 +206,8 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 // weight gradients from the codes:  dW[m][k] = sum_r dy[r][m] x^[r][k],   db[m] = sum_r dy[r][m]
 //
 // A code with its scale has four significant bits: it is a bf16 number, exactly.  dy is written as a sum of bf16 numbers, exactly too: one for
-// bf16, two for fp16 (11 bits), three for fp32 (24 bits; each the truncation of what is left, so that no rounding can overflow; only what lies below 2^-133, bf16's smallest number, is
-// lost).  So 1 / 2 / 3
-// bf16 matrix instructions with fp32 accumulation give every product exactly, at 16 / 8 / 5.3 times the fp32 matrix rate: the result is that
+// bf16, two for fp16 (11 bits), three for fp32 (24 bits; each the truncation of what is left, so that no rounding can overflow; only what lies below 2^-133, bf16's smallest
+// number, is lost).  So 1 / 2 / 3 bf16 matrix instructions with fp32 accumulation give every product exactly, at 16 / 8 / 5.3 times the fp32 matrix rate: the result is that
 // of an fp32 product of dy with the unpacked values, up to the order of the sums.
 //
 // Both operands lie along the outputs, and the reduction runs over the rows: a wave loads 8 rows, a lane C adjacent columns of them, and 8 rows of
@@ -218,6 +219,11 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 // packed into the other and the one after that is on its way in registers; one barrier a slab.  C = 4 (256 x 256: 64 matrix instructions a
 // slab and plane for 32 fragment reads) where that fills the chip, else C = 2 (two workgroups a CU).  The rows are split into slices, whose
 // partial tiles a second launch adds in a fixed order.
+//
+// What bounds it: 32 768 rows, 2 048 x 2 048, bf16: 294 us = 935 TFLOP/s (the library's 8192^3 bf16 product reaches 1 093), the matrix unit busy 47 % of
+// the cycles at the clock that its power leaves, 28 % of a wave's cycles waiting (fragments out of LDS: 96 KB a slab and workgroup).
+// 63 001 rows, 256 x 256, fp32 (three planes): 48 us for 81 MB of operands (each read by two tiles) and 24.8 GFLOP in bf16.  Neither bound is
+// near (16 us, 23 us): 124 slices of four tiles leave a workgroup 16 slabs, of which the first and the last three run unoverlapped.
 // ------------------------------------------------------------------------------------------------
 #define A8_MAX_JOBS 16
 #define A8_SLAB 32
@@ -484,6 +490,7 @@ __global__ void __launch_bounds__(256, C == 4 ? 1 : 2) k_act8_wgrad(A8Args a, A8
 }
 
 // Slices added in a fixed order: a thread a quarter of them for four numbers, then the four quarters.  Record: [weights (n_w) | biases].
+// (124 slices of 65 792 numbers, 33 MB: 10 us; 4 of 4.2 million, 84 MB: 14 us.)
 __global__ void __launch_bounds__(256) k_act8_fold(const float* __restrict__ part, long long n, long long n_w, long long n_all, int nslices, float* __restrict__ dw,
                                                    float* __restrict__ db)
 {

@@ -212,7 +212,8 @@ extern "C" int nf_scan_fwd(const nf_scan_t* s, nf_stream_t stream) { return scan
 extern "C" int nf_scan_bwd(const nf_scan_t* s, nf_stream_t stream) { return scan_run(s, 1, (hipStream_t)stream, __func__); }
 
 // ------------------------------------------------------------------------------------------------
-// one step: next = A state + x, h = next rounded to the storage type.  Reads gate, x and state, writes both: bandwidth, or the launch.
+// one step: next = A state + x, h = next rounded to the storage type.  Reads gate, x and state, writes both: bandwidth, or the launch
+// (160 000 x 64 bf16, 144 MB: 21.9 us, 6.6 TB/s; 1 024 x 32 fp32: 2.9 us).
 // ------------------------------------------------------------------------------------------------
 struct NfStepArgs {
     const void* gate; const void* x; const float* state; float* next; void* h;
