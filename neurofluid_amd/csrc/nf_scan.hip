@@ -79,36 +79,49 @@ extern "C" size_t nf_scan_workspace_bytes(const nf_scan_t* s, int backward)
     return 8 * scan_workspace(s, backward).words();
 }
 
-// The sequence of every packed row (-1: before the first or behind the last), by bisection of the splits; the final states of empty
-// sequences are their initial ones (and their gradients pass through): written here.  Splits are clamped to [0, T], so that bad ones give bad
-// numbers but no access out of range.
-__global__ void __launch_bounds__(256) k_scan_rows(const int64_t* __restrict__ rs, int n_seq, int T, int* __restrict__ sid)
+// What has to be there before the tiles run, in one launch (any part may be absent; as three launches: 164 us for
+// 50 001 packed rows of 200 channels with gradients instead of 157).
+//  - The sequence of every packed row (-1: before the first or behind the last), by bisection of the splits.
+//  - The final states of empty sequences are their initial ones (and their gradients pass through).  Splits are clamped to [0, T], so that bad ones
+//    give bad numbers but no access out of range.
+//  - The chain's entries are set to "empty", the counters of tiles to 0 (by a kernel: a memset node in a captured graph has given wrong results).
+struct NfFront {
+    const int64_t* rs; int n_seq, T, D;
+    int* sid;                                            // rows, or NULL
+    const float* src; float* dst;                        // empty sequences: from src (NULL: zeros), or dst NULL
+    unsigned long long* words; size_t entries, n;        // the workspace's
+};
+__global__ void __launch_bounds__(256) k_scan_front(NfFront a)
 {
-    const int r = blockIdx.x * 256 + threadIdx.x;
-    if (r >= T) return;
-    int lo = 0, hi = n_seq;              // the number of k in [1, n_seq] with rs[k] <= r
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (rs[mid + 1] <= r) lo = mid + 1;
-        else hi = mid;
-    }
-    sid[r] = (lo < n_seq && rs[lo] <= r) ? lo : -1;
+    const size_t first = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
+    for (size_t i = first; i < a.n; i += step) a.words[i] = i < a.entries ? NF_SCAN_EMPTY : 0ull;
+    if (a.sid)
+        for (size_t r = first; r < (size_t)a.T; r += step) {
+            int lo = 0, hi = a.n_seq;            // the number of k in [1, n_seq] with rs[k] <= r
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (a.rs[mid + 1] <= (int64_t)r) lo = mid + 1;
+                else hi = mid;
+            }
+            a.sid[r] = (lo < a.n_seq && a.rs[lo] <= (int64_t)r) ? lo : -1;
+        }
+    if (a.dst)
+        for (size_t e = first; e < (size_t)a.n_seq * a.D; e += step) {
+            const int s = (int)(e / a.D);
+            const int64_t b0 = min(max(a.rs[s], (int64_t)0), (int64_t)a.T), b1 = min(max(a.rs[s + 1], (int64_t)0), (int64_t)a.T);
+            if (b0 >= b1) a.dst[e] = a.src ? a.src[e] : 0.f;
+        }
 }
-
-__global__ void __launch_bounds__(256) k_scan_empty(const int64_t* __restrict__ rs, int n_seq, int T, int D, const float* __restrict__ src,
-                                                    float* __restrict__ dst)
+static int scan_front(const NfFront& f, hipStream_t st)
 {
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < (long long)n_seq * D; e += (long long)gridDim.x * 256) {
-        const int s = (int)(e / D);
-        const int64_t a = min(max(rs[s], (int64_t)0), (int64_t)T), b = min(max(rs[s + 1], (int64_t)0), (int64_t)T);
-        if (a >= b) dst[e] = src ? src[e] : 0.f;
-    }
-}
-
-// The chain's entries are set to "empty", the counters of tiles to 0 (a kernel: a memset node in a captured graph has given wrong results).
-__global__ void __launch_bounds__(256) k_scan_clear(unsigned long long* __restrict__ w, size_t entries, size_t n)
-{
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) w[i] = i < entries ? NF_SCAN_EMPTY : 0ull;
+    size_t n = f.n;
+    if (f.sid && (size_t)f.T > n) n = f.T;
+    if (f.dst && (size_t)f.n_seq * f.D > n) n = (size_t)f.n_seq * f.D;
+    if (n == 0) return NF_OK;
+    const size_t blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(k_scan_front, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, f);
+    NF_CHECK_LAUNCH();
+    return NF_OK;
 }
 
 __global__ void __launch_bounds__(256) k_scan_fold(const float* __restrict__ part, int nblk, long long n, int type, void* __restrict__ out)
@@ -139,12 +152,12 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     const float* init = backward ? s->g_last : s->h0;
     float* fin = backward ? s->dh0 : s->h_last;
     if (!backward && !fin && n_state > 0) { nf_set_error("%s: null h_last", who); return NF_EINVAL; }
-    if (packed && s->n_seq > 0 && fin) {
-        const long long blocks = ((long long)s->n_seq * s->D + 255) / 256;
-        hipLaunchKernelGGL(k_scan_empty, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->D, init, fin);
-        NF_CHECK_LAUNCH();
+    NfFront front = {};
+    if (packed) {
+        front.rs = s->row_splits; front.n_seq = s->n_seq; front.T = s->T; front.D = s->D;
+        front.src = init; front.dst = fin;
     }
-    if (s->B == 0 || s->T == 0) return NF_OK;        // (dense with T = 0: the caller copies the state)
+    if (s->B == 0 || s->T == 0) return scan_front(front, st);        // (dense with T = 0: the caller copies the state)
     if (!s->gate || !s->x || (backward ? !s->states : !s->h)) { nf_set_error("%s: null pointer", who); return NF_EINVAL; }
     if (packed && !s->sid) { nf_set_error("%s: packed rows need the row buffer (sid)", who); return NF_EINVAL; }
     const int es = s->dtype == 0 ? 4 : 2, gs = (s->dtype == 0 || s->gate32) ? 4 : 2;
@@ -185,15 +198,10 @@ static int scan_run(const nf_scan_t* s, int backward, hipStream_t st, const char
     unsigned long long* words = (unsigned long long*)s->workspace;
     a.ws_tile = words; a.ws_group = words + ws.tile; a.ws_set = a.ws_group + ws.group; a.ticket = (int*)(words + ws.entries());
     a.dgate_part = n_part ? (float*)(words + ws.entries() + ws.counters) : nullptr;
-    if (packed && !backward) {
-        hipLaunchKernelGGL(k_scan_rows, dim3((unsigned)((s->T + 255) / 256)), dim3(256), 0, st, s->row_splits, s->n_seq, s->T, s->sid);
-        NF_CHECK_LAUNCH();
-    }
-    if (ws.entries()) {
-        const size_t n = ws.entries() + ws.counters, blocks = (n + 255) / 256;
-        hipLaunchKernelGGL(k_scan_clear, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, st, words, ws.entries(), n);
-        NF_CHECK_LAUNCH();
-    }
+    if (packed && !backward) front.sid = s->sid;
+    front.words = words; front.entries = ws.entries(); front.n = ws.entries() + ws.counters;
+    const int rf = scan_front(front, st);
+    if (rf) return rf;
     for (long long c = 0; c < chains; c += s->mode == NF_SCAN_WAVE ? NF_SCAN_SLICE : chains) {
         a.chain0 = (int)c;
         if (!scan_go(s, a, backward, st)) { nf_set_error("%s: no kernel for the plan", who); return NF_EINVAL; }
