@@ -176,6 +176,8 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
         if row_splits.dtype != torch.int64 or row_splits.dim() != 1 or row_splits.numel() < 1 or row_splits.device != x.device:
             raise ValueError(f"{what}: row_splits must be a non-empty 1-d int64 tensor on {x.device}")
         row_splits = row_splits.contiguous()
+        if row_splits.numel() > _MAX_STEPS:
+            raise ValueError(f"{what}: more than {_MAX_STEPS} sequences")
     if x.shape[-2] > _MAX_STEPS or (not packed and x.shape[0] > _MAX_STEPS) or x.shape[-1] > _MAX_CHANNELS:
         raise ValueError(f"{what}: more than {_MAX_STEPS} steps or sequences, or than {_MAX_CHANNELS} channels")
     if h0 is not None:
