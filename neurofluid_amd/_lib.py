@@ -242,7 +242,7 @@ def on_device(fn):
     @functools.wraps(fn)
     def call(t, *args, **kw):
         dev = t.get_device()
-        if dev < 0 or dev == torch.cuda.current_device():
+        if dev < 0 or dev == torch._C._cuda_getDevice():         # (t is on a GPU: torch.cuda is initialised)
             return fn(t, *args, **kw)
         with torch.cuda.device(dev):
             return fn(t, *args, **kw)

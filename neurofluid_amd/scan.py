@@ -26,15 +26,16 @@ def _rows(t):
 
 
 def _check(gate, x, what):
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"{what}: x must be float32, bfloat16 or float16, not {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"{what}: x needs an axis of steps or rows and one of channels, got {tuple(x.shape)}")
-    if gate.dtype not in (x.dtype, torch.float32):
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _DTYPES:
+        raise TypeError(f"{what}: x must be float32, bfloat16 or float16, not {dtype}")
+    if len(shape) < 2:
+        raise ValueError(f"{what}: x needs an axis of steps or rows and one of channels, got {tuple(shape)}")
+    if gate.dtype is not dtype and gate.dtype is not torch.float32:
         raise TypeError(f"{what}: the gate must have x's dtype or float32, not {gate.dtype}")
-    if gate.shape != x.shape and (gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.shape[-1] != 1):
-        raise ValueError(f"{what}: gate {tuple(gate.shape)} does not fit x {tuple(x.shape)} (same shape, or one gate a step: last axis 1)")
-    if x.shape[-1] < 1:
+    if gate.shape != shape and (gate.dim() != len(shape) or gate.shape[:-1] != shape[:-1] or gate.shape[-1] != 1):
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} does not fit x {tuple(shape)} (same shape, or one gate a step: last axis 1)")
+    if shape[-1] < 1:
         raise ValueError(f"{what}: x has no channels")
     if gate.device != x.device:
         raise ValueError(f"{what}: gate and x are on different devices")
@@ -199,19 +200,22 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
         raise ValueError(f"{what}: x must be (rows, D), got {tuple(x.shape)}")
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
         raise RuntimeError(f"{what} carries no gradients (use gated_scan, or torch.no_grad())")
-    rows, D = x.shape
-    span = []
-    for t, name in ((state, "state"),) if out is None else ((state, "state"), (out, "out")):
-        _check_state(t, x.shape, x, what, name)
-        s0, s1 = t.stride()
-        if (D > 1 and s1 != 1) or (rows > 1 and s0 < D):
-            raise ValueError(f"{what}: {name} needs adjacent channels and rows that do not overlap")
-        span.append((t.data_ptr(), s0, 4 * ((rows - 1) * s0 + D)))
-    (a, sa, na), (b, sb, nb) = span[0], span[-1]
+    shape = x.shape
+    rows, D = shape
+    a, sa, na = _states(state, shape, rows, D, x, what, "state")
+    b, sb, nb = (a, sa, na) if out is None else _states(out, shape, rows, D, x, what, "out")
     if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na:
         raise ValueError(f"{what}: out overlaps state without being it")
     ops._require_cuda(gate, x)
-    return _step(x, gate, a, sa, b, sb, log_gate)
+    return _step(x, gate, a, sa, b, sb, rows, D, bool(log_gate))
+
+
+def _states(t, shape, rows, D, x, what, name):
+    _check_state(t, shape, x, what, name)
+    s0, s1 = t.stride()
+    if (D > 1 and s1 != 1) or (rows > 1 and s0 < D):
+        raise ValueError(f"{what}: {name} needs adjacent channels and rows that do not overlap")
+    return t.data_ptr(), s0, 4 * ((rows - 1) * s0 + D)
 
 
 def _apart(t, out, out_stride, rows, D):
@@ -225,19 +229,26 @@ def _apart(t, out, out_stride, rows, D):
 
 
 @_lib.on_device
-def _step(x, gate, state, state_stride, out, out_stride, log_gate):
-    rows, D = x.shape
-    g_, x_ = _rows(gate), _rows(x)
-    gp, gs, xp, xs = g_.data_ptr(), g_.stride(0), x_.data_ptr(), x_.stride(0)
+def _step(x, gate, state, state_stride, out, out_stride, rows, D, log_gate):
+    (gs, g1), (xs, x1) = gate.stride(), x.stride()
+    shared = gate.shape[1] == 1
+    if (g1 != 1 and not shared) or gs > _MAX_STRIDE:
+        gate = _rows(gate)
+        gs = gate.stride(0)
+    if x1 != 1 or xs > _MAX_STRIDE:
+        x = _rows(x)
+        xs = x.stride(0)
+    gp, xp = gate.data_ptr(), x.data_ptr()
     end = out + 4 * (rows * out_stride + D)            # (generous bounds; _apart looks closer)
     if gp < end and out < gp + 4 * (rows * gs + D):
-        g_ = _apart(g_, out, out_stride, rows, D)
-        gp, gs = g_.data_ptr(), g_.stride(0)
+        gate = _apart(gate, out, out_stride, rows, D)
+        gp, gs = gate.data_ptr(), gate.stride(0)
     if xp < end and out < xp + 4 * (rows * xs + D):
-        x_ = _apart(x_, out, out_stride, rows, D)
-        xp, xs = x_.data_ptr(), x_.stride(0)
-    h = torch.empty((rows, D), dtype=x.dtype, device=x.device)
+        x = _apart(x, out, out_stride, rows, D)
+        xp, xs = x.data_ptr(), x.stride(0)
+    dtype = x.dtype
+    h = torch.empty_like(x) if xs == D and x1 == 1 else torch.empty((rows, D), dtype=dtype, device=x.device)       # (the former in half the time)
     if rows:
-        check(_lib.load().nf_scan_step(_DTYPES[x.dtype], gate.dtype is torch.float32, gate.shape[1] == 1, bool(log_gate), rows, D, gp, gs, xp, xs,
-                                       state, state_stride, out, out_stride, h.data_ptr(), _lib.raw_stream(x)), "nf_scan_step")
+        check(_lib.load().nf_scan_step(_DTYPES[dtype], gate.dtype is torch.float32, shared, log_gate, rows, D, gp, gs, xp, xs, state, state_stride,
+                                       out, out_stride, h.data_ptr(), _lib.raw_stream(x)), "nf_scan_step")
     return h
