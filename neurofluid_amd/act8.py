@@ -7,6 +7,7 @@ Forward values and the gradients of the inputs are those of the exact activation
 There is no torch fallback: CPU tensors raise.
 """
 import ctypes
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -24,6 +25,12 @@ def _matrix(t):
     return m if m.shape[1] <= 1 or m.stride(1) == 1 else m.contiguous()
 
 
+def _sizes(rows, features):
+    """Bytes of the codes and of the scales (nf_act8_code_bytes, nf_act8_scale_bytes)."""
+    blocks = (features + 31) // 32
+    return 32 * rows * blocks, (rows + 63) // 64 * 64 * blocks
+
+
 class Act8:
     """A matrix in 8 bits: ``codes`` and ``scales`` (uint8, the layout of nf_act8_pack), ``shape`` and ``dtype`` of what was packed."""
 
@@ -36,10 +43,7 @@ class Act8:
 
     @property
     def rows(self):
-        n = 1
-        for k in self.shape[:-1]:
-            n *= k
-        return n
+        return math.prod(self.shape[:-1])
 
     @property
     def device(self):
@@ -47,10 +51,12 @@ class Act8:
 
     def _whole(self, what):
         """The kernels read what the shape says: refuse less."""
-        rows, blocks = self.rows, (self.features + 31) // 32
-        for t, n, name in ((self.codes, 32 * rows * blocks, "codes"), (self.scales, (rows + 63) // 64 * 64 * blocks, "scales")):
-            if t.dtype is not torch.uint8 or t.numel() < n or not t.is_contiguous() or t.device != self.codes.device:
-                raise ValueError(f"{what}: {name} of {self.shape} must be {n} adjacent bytes on one device, got {t.dtype} {tuple(t.shape)}")
+        codes, scales = self.codes, self.scales
+        sizes = _sizes(self.rows, self.shape[-1])
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.numel() < sizes[0] or scales.numel() < sizes[1] or \
+                not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
+            raise ValueError(f"{what}: codes and scales of {self.shape} must be {sizes} adjacent bytes (uint8) on one device, got {codes.dtype} "
+                             f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
 
     @property
     def tensors(self):
@@ -85,21 +91,23 @@ def pack(x):
 
 @_lib.on_device
 def _pack(x, rows):
-    lib = _lib.load()
-    K = x.shape[-1]
-    m = _matrix(x.detach()) if rows else x.detach()
-    n_codes = lib.nf_act8_code_bytes(rows, K)         # (a multiple of 32)
-    both = torch.empty(n_codes + lib.nf_act8_scale_bytes(rows, K), dtype=torch.uint8, device=x.device)
-    codes, scales = both[:n_codes], both[n_codes:]
-    if rows and K:
-        check(lib.nf_act8_pack(_DTYPES[x.dtype], m.data_ptr(), m.stride(0), rows, K, codes.data_ptr(), scales.data_ptr(), _lib.raw_stream(x)), "nf_act8_pack")
-    return Act8(codes, scales, x.shape, x.dtype)
+    shape = x.shape
+    K, sizes = shape[-1], _sizes(rows, shape[-1])
+    n_codes, n_scales = sizes                         # (multiples of 32)
+    both = torch.empty(n_codes + n_scales, dtype=torch.uint8, device=x.device)
+    if n_codes:
+        m = x if len(shape) == 2 and x.stride(1) == 1 else _matrix(x.detach())
+        p = both.data_ptr()
+        check(_lib.load().nf_act8_pack(_DTYPES[x.dtype], m.data_ptr(), m.stride(0), rows, K, p, p + n_codes, _lib.raw_stream(x)), "nf_act8_pack")
+    codes, scales = both.split_with_sizes(sizes)
+    return Act8(codes, scales, shape, x.dtype)
 
 
 @_lib.on_device
 def _unpack(codes, ck, dtype):
     out = torch.empty(ck.shape, dtype=dtype, device=codes.device)
-    check(_lib.load().nf_act8_unpack(_DTYPES[dtype], codes.data_ptr(), ck.scales.data_ptr(), ck.rows, ck.features, out.data_ptr(), ck.features,
+    K = ck.shape[-1]
+    check(_lib.load().nf_act8_unpack(_DTYPES[dtype], codes.data_ptr(), ck.scales.data_ptr(), ck.rows, K, out.data_ptr(), K,
                                      _lib.raw_stream(codes)), "nf_act8_unpack")
     return out
 

@@ -45,6 +45,16 @@ def test_a_checkpoint_that_is_not_whole_is_refused():
     act8.Act8(whole.codes, t(256, dtype=torch.uint8), (70, 40), torch.float32)._whole("here")
 
 
+@pytest.mark.parametrize("rows", [0, 1, 63, 64, 65, 1000])
+@pytest.mark.parametrize("K", [0, 1, 31, 32, 33, 2432])
+def test_sizes_are_the_c_entries(rows, K):
+    from neurofluid_amd import _lib, build
+    build.build()
+    lib = _lib.load()
+    want = (lib.nf_act8_code_bytes(rows, K), lib.nf_act8_scale_bytes(rows, K))
+    assert act8._sizes(rows, K) == want
+
+
 def test_unpack_refuses():
     with pytest.raises(TypeError):
         fake(2, 3).unpack(torch.float64)
