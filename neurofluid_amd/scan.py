@@ -193,12 +193,13 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
 def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
     """One step for every row: the new state A * state + x goes to ``out`` (by default into ``state`` itself), its value in x's dtype is returned.
 
-    x: (rows, D); gate: x's shape or (rows, 1); state, out: (rows, D) float32 with adjacent channels.  x and gate may lie in the same memory.  For inference: no gradients."""
+    x: (rows, D); gate: x's shape or (rows, 1); state, out: (rows, D) float32 with adjacent channels.  x and gate may lie in the same memory.  For inference: no gradients.
+    What is written counts as changed in place: a backward that still needs the old state refuses to run."""
     what = "gated_scan_step"
     _check(gate, x, what)
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be (rows, D), got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad or (out is not None and out.requires_grad)):
         raise RuntimeError(f"{what} carries no gradients (use gated_scan, or torch.no_grad())")
     shape = x.shape
     rows, D = shape
@@ -207,7 +208,10 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
     if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na:
         raise ValueError(f"{what}: out overlaps state without being it")
     ops._require_cuda(gate, x)
-    return _step(x, gate, a, sa, b, sb, rows, D, bool(log_gate))
+    h = _step(x, gate, a, sa, b, sb, rows, D, bool(log_gate))
+    # the kernel writes through the pointer, which autograd's check of saved tensors and caches keyed on the version would not see
+    torch.autograd.graph.increment_version(state if out is None else out)
+    return h
 
 
 def _states(t, shape, rows, D, x, what, name):

@@ -519,3 +519,21 @@ def test_composites_like_the_renderer(dev):
     # 192 samples of magnitude <= 5 with weights that sum to <= 1; 8 u a step as above
     assert (h[:, 0].cpu().double() - want).abs().max() <= 8 * 192 * U * 5
     assert torch.equal(h[:, 0], last)
+
+
+def test_a_step_behind_a_recorded_scan_is_noticed(dev):
+    """The scan's backward reads h0 again: a step that writes there in between makes it refuse, a step into memory of its own does not."""
+    from neurofluid_amd import scan
+    gate, x, gy, gen = make((2, 40, 8), (2, 40, 8), F32, F32, False, 6)
+    g0, x0, y0, s0 = gate.to(dev).requires_grad_(), x.to(dev), gy.to(dev), torch.randn(2, 8, generator=gen).to(dev)
+
+    def run(step):
+        s = s0.clone()
+        h, last = scan.gated_scan(g0, x0, s)
+        with torch.no_grad():
+            step(s)
+        return torch.autograd.grad(h, g0, y0)[0]
+    want = run(lambda s: None)
+    assert torch.equal(run(lambda s: scan.gated_scan_step(x0[:, 0], x0[:, 1], s, out=torch.empty_like(s))), want)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        run(lambda s: scan.gated_scan_step(x0[:, 0], x0[:, 1], s))

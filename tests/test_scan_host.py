@@ -92,3 +92,45 @@ def test_the_packed_descriptor_is_the_struct():
     scan._PACK.pack_into(buf, 0, *range(1, len(names) + 1))
     s = _lib.Scan.from_buffer(buf)
     assert [getattr(s, n) for n in names] == list(range(1, len(names) + 1))
+
+
+@pytest.fixture
+def no_gpu(monkeypatch):
+    """The host side on CPU tensors: the C entries note what they are given and do nothing."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            def entry(*args):
+                calls.append((name, args))
+                return 0
+            return entry
+    lib = Lib()
+    monkeypatch.setattr(scan._lib, "load", lambda: lib)
+    monkeypatch.setattr(scan._lib, "raw_stream", lambda q: 0)
+    monkeypatch.setattr(scan.ops, "_require_cuda", lambda *a: None)
+    return calls
+
+
+@pytest.mark.parametrize("own_out", [False, True])
+def test_step_counts_as_a_change_in_place(no_gpu, own_out):
+    """A recorded operation that keeps the state refuses its backward once a step has written there, as after any in-place operation."""
+    w, s = torch.ones(4, 3, requires_grad=True), t(4, 3)
+    y, before = (w * s).sum(), s._version
+    with torch.no_grad():
+        scan.gated_scan_step(t(4, 3), t(4, 3), t(4, 3) if own_out else s, **(dict(out=s) if own_out else {}))
+    assert no_gpu and s._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # ... seen through a view too; a state that is only read stays as it was
+    rows, read = t(8, 5), t(4, 3)
+    before = rows._version, read._version
+    scan.gated_scan_step(t(4, 3), t(4, 3), read, out=rows[::2, 1:4])
+    assert (rows._version, read._version) == (before[0] + 1, before[1])
+    with torch.inference_mode():
+        scan.gated_scan_step(t(4, 3), t(4, 3), t(4, 3))
+
+
+def test_step_refuses_an_out_with_gradients():
+    with pytest.raises(RuntimeError, match="no gradients"):
+        scan.gated_scan_step(t(4, 3), t(4, 3), t(4, 3), out=t(4, 3).requires_grad_())
