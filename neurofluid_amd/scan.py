@@ -16,6 +16,7 @@ from ._lib import check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX_STEPS, _MAX_CHANNELS, _MAX_STRIDE = 1 << 30, 1 << 20, 1 << 17
+_INT_MAX = (1 << 31) - 1            # what the C entry takes (ctypes would keep a larger number's low 32 bits)
 
 
 def _rows(t):
@@ -203,6 +204,8 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
         raise RuntimeError(f"{what} carries no gradients (use gated_scan, or torch.no_grad())")
     shape = x.shape
     rows, D = shape
+    if rows > _INT_MAX or D > _INT_MAX:
+        raise ValueError(f"{what}: more than {_INT_MAX} rows or channels")
     a, sa, na = _states(state, shape, rows, D, x, what, "state")
     b, sb, nb = (a, sa, na) if out is None else _states(out, shape, rows, D, x, what, "out")
     if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na:

@@ -134,3 +134,16 @@ def test_step_counts_as_a_change_in_place(no_gpu, own_out):
 def test_step_refuses_an_out_with_gradients():
     with pytest.raises(RuntimeError, match="no gradients"):
         scan.gated_scan_step(t(4, 3), t(4, 3), t(4, 3), out=t(4, 3).requires_grad_())
+
+
+@pytest.mark.parametrize("rows, D", [(2 ** 32, 1), (2 ** 32 + 5, 1), (2 ** 31, 1), (1, 2 ** 31)])
+def test_step_refuses_sizes_that_the_c_entry_would_cut(no_gpu, rows, D):
+    """(Views and storage that is never touched: no memory behind it.)"""
+    x = t(1, 1, dtype=torch.bfloat16).expand(rows, D)
+    state = torch.empty(rows, D, device="meta")
+
+    class OnTheCpu(torch.Tensor):
+        device = torch.device("cpu")
+    with pytest.raises(ValueError, match="more than"):
+        scan.gated_scan_step(x, x, state.as_subclass(OnTheCpu))
+    assert not no_gpu
