@@ -208,7 +208,8 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
         raise ValueError(f"{what}: more than {_INT_MAX} rows or channels")
     a, sa, na = _states(state, shape, rows, D, x, what, "state")
     b, sb, nb = (a, sa, na) if out is None else _states(out, shape, rows, D, x, what, "out")
-    if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na:
+    if (a != b or (sa != sb and rows > 1)) and a < b + nb and b < a + na and not (rows > 1 and sa == sb and 4 * D <= (b - a) % (4 * sa) <= 4 * (sa - D)):
+        # (the last: rows equally far apart, out's columns beside the state's in every one of them)
         raise ValueError(f"{what}: out overlaps state without being it")
     ops._require_cuda(gate, x)
     h = _step(x, gate, a, sa, b, sb, rows, D, bool(log_gate))

@@ -537,3 +537,20 @@ def test_a_step_behind_a_recorded_scan_is_noticed(dev):
     assert torch.equal(run(lambda s: scan.gated_scan_step(x0[:, 0], x0[:, 1], s, out=torch.empty_like(s))), want)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         run(lambda s: scan.gated_scan_step(x0[:, 0], x0[:, 1], s))
+
+
+def test_step_into_the_columns_beside_the_state(dev):
+    """State and out as column ranges of one buffer, either way round; what lies between and behind them stays."""
+    from neurofluid_amd import scan
+    g = torch.Generator().manual_seed(23)
+    for D, width, first, second in ((64, 128, 0, 64), (5, 13, 8, 1), (64, 136, 68, 0)):
+        base, x = torch.randn(300, width, generator=g), torch.randn(300, D, generator=g)
+        gate = torch.rand(300, D, generator=g)
+        buf = base.to(dev)
+        h = scan.gated_scan_step(gate.to(dev), x.to(dev), buf[:, first:first + D], out=buf[:, second:second + D])
+        state = base[:, first:first + D].double()
+        assert ((h.cpu().double() - (gate.double() * state + x.double())).abs() <= 4 * U * ((gate * state).abs() + x.abs())).all()
+        assert torch.equal(buf[:, second:second + D], h)
+        rest = torch.ones(width, dtype=torch.bool)
+        rest[second:second + D] = False
+        assert torch.equal(buf.cpu()[:, rest], base[:, rest])

@@ -147,3 +147,30 @@ def test_step_refuses_sizes_that_the_c_entry_would_cut(no_gpu, rows, D):
     with pytest.raises(ValueError, match="more than"):
         scan.gated_scan_step(x, x, state.as_subclass(OnTheCpu))
     assert not no_gpu
+
+
+def test_step_takes_an_out_beside_the_state_in_the_same_rows(no_gpu):
+    """The check of overlaps against a comparison of every address, over all pairs of windows of one buffer."""
+    x = t(3, 2)
+    buf = t(60)
+    taken = refused = 0
+    for stride_a in (2, 3, 5):
+        for stride_b in (2, 3, 5):
+            for at_a in range(0, 30, 7):
+                for at_b in range(0, 40):
+                    state, out = buf.as_strided((3, 2), (stride_a, 1), at_a), buf.as_strided((3, 2), (stride_b, 1), at_b)
+                    where = lambda base, st: {base + r * st + c for r in range(3) for c in range(2)}
+                    same, apart = (at_a, stride_a) == (at_b, stride_b), not where(at_a, stride_a) & where(at_b, stride_b)
+                    if same or (apart and stride_a == stride_b):
+                        scan.gated_scan_step(x, x, state, out=out)
+                        taken += 1
+                    elif not apart:
+                        with pytest.raises(ValueError, match="overlaps"):
+                            scan.gated_scan_step(x, x, state, out=out)
+                        refused += 1
+    assert taken > 100 and refused > 100
+    one = buf.as_strided((1, 2), (0, 1), 1)               # (one row: any stride)
+    with pytest.raises(ValueError, match="overlaps"):
+        scan.gated_scan_step(t(1, 2), t(1, 2), buf[None, :2], out=one)
+    with pytest.raises(ValueError, match="overlaps"):
+        scan.gated_scan_step(t(1, 2), t(1, 2), buf.as_strided((1, 2), (0, 1), 0), out=one)
