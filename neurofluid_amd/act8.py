@@ -72,6 +72,7 @@ class Act8:
         if dtype not in _DTYPES:
             raise TypeError(f"Act8.unpack: float32, bfloat16 or float16, not {dtype}")
         self._whole("Act8.unpack")
+        ops._require_cuda(self.codes)
         return _unpack(self.codes, self, dtype)
 
 

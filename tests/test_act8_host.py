@@ -100,3 +100,12 @@ def test_c_entries_refuse():
     assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 0, ok, None, None, None, None) < 0
     assert lib.nf_act8_wgrad(0, None, 4, 4, None, None, 64, 8, 1, ok, None, None, None, None) < 0 and b"null" in lib.nf_last_error()
     assert lib.nf_act8_wgrad_workspace_floats(100000, 4, 64, 1, ok) > 0
+
+
+def test_codes_in_host_memory_are_refused():
+    """A whole checkpoint that was moved to the host: its pointers are not the GPU's to read."""
+    ck = act8.Act8(t(70 * 64, dtype=torch.uint8), t(256, dtype=torch.uint8), (70, 40), torch.float32)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        ck.unpack()
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        act8.wgrad(t(70, 4), ck)
