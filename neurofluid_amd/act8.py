@@ -87,6 +87,7 @@ def pack(x):
     if rows > _MAX or x.shape[-1] > _MAX:
         raise ValueError(f"act8.pack: more than {_MAX} rows or features")
     ops._require_cuda(x)
+    ops._refuse_tangents("act8.pack", x)
     return _pack(x, rows)
 
 
@@ -127,6 +128,7 @@ def wgrad_jobs(dy, ckpt, jobs):
     if not 1 <= len(jobs) <= 16:
         raise ValueError("act8.wgrad: 1 to 16 jobs")
     ops._require_cuda(dy)
+    ops._refuse_tangents("act8.wgrad", dy)
     if dy.device != ckpt.device:
         raise ValueError("act8.wgrad: dy and the activations are on different devices")
     ckpt._whole("act8.wgrad")
@@ -183,6 +185,7 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        ops._refuse_tangents("act8.linear's backward", g)
         weight, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
@@ -203,7 +206,7 @@ class _LinearFn(torch.autograd.Function):
 
 def linear(x, weight, bias=None):
     """torch.nn.functional.linear on float32 whose input is kept in 8 bits for the backward (4.1 times fewer bytes): y = x W^T + b and dx = dy W run
-    on the fp32 matrix pipe (ops.gemm), dW and db are ``wgrad`` of the packed input.  Differentiable once."""
+    on the fp32 matrix pipe (ops.gemm), dW and db are ``wgrad`` of the packed input.  Differentiable once, in reverse mode."""
     for t, name, dims in ((x, "x", None), (weight, "weight", 2), (bias, "bias", 1)):
         if t is None:
             continue
@@ -217,6 +220,7 @@ def linear(x, weight, bias=None):
     if any(t is not None and t.device != x.device for t in (weight, bias)):
         raise ValueError("act8.linear: x, weight and bias are on different devices")
     ops._require_cuda(x)
+    ops._refuse_tangents("act8.linear", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LinearFn.apply(x, weight, bias)
     return _linear(x, weight, bias)[0]

@@ -11,6 +11,7 @@ import os
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr
@@ -33,6 +34,12 @@ def _require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("neurofluid_amd ops need tensors on the GPU (no CPU fallback)")
+
+
+def _refuse_tangents(what, *ts):
+    """For entry points that read tensors through their pointers: a dual tensor's is its primal's, and the tangent would be lost unseen."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 # ------------------------------------------------------------------------------------------------

@@ -126,6 +126,7 @@ class _ScanFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, g_last):
+        ops._refuse_tangents("gated_scan's backward", g, g_last)
         gate, x, h0, row_splits, states, sid = ctx.saved_tensors
         return _backward(x, gate, h0, row_splits, states, sid, g, g_last, ctx.opts, ctx.plan, ctx.needs_input_grad) + (None, None)
 
@@ -168,7 +169,7 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     rows that belong to no sequence.
 
     Sums, states and the carries between stretches are float32; h is rounded once.  Gates are meant to be decays, |A| <= 1: products of larger ones over long
-    stretches overflow, and where a product of gates has reached zero an infinite state goes on as NaN.  Differentiable once in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
+    stretches overflow, and where a product of gates has reached zero an infinite state goes on as NaN.  Differentiable once, in reverse mode, in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
     what = "gated_scan"
     _check(gate, x, what)
     packed = row_splits is not None
@@ -185,6 +186,7 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     if h0 is not None:
         _check_state(h0, (row_splits.numel() - 1 if packed else x.shape[0], x.shape[-1]), x, what, "h0")
     ops._require_cuda(gate, x)
+    ops._refuse_tangents(what, gate, x, h0)
     opts = (bool(log_gate), bool(reverse))
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
         return _ScanFn.apply(gate, x, h0, row_splits, opts)
@@ -212,6 +214,7 @@ def gated_scan_step(gate, x, state, *, log_gate=False, out=None):
         # (the last: rows equally far apart, out's columns beside the state's in every one of them)
         raise ValueError(f"{what}: out overlaps state without being it")
     ops._require_cuda(gate, x)
+    ops._refuse_tangents(what, gate, x, state, out)
     h = _step(x, gate, a, sa, b, sb, rows, D, bool(log_gate))
     # the kernel writes through the pointer, which autograd's check of saved tensors and caches keyed on the version would not see
     torch.autograd.graph.increment_version(state if out is None else out)

@@ -109,3 +109,16 @@ def test_codes_in_host_memory_are_refused():
         ck.unpack()
     with pytest.raises(RuntimeError, match="on the GPU"):
         act8.wgrad(t(70, 4), ck)
+
+
+def test_forward_mode_is_refused(monkeypatch):
+    from torch.autograd import forward_ad as fw
+    monkeypatch.setattr(act8.ops, "_require_cuda", lambda *a: None)
+    ck = act8.Act8(t(4 * 32, dtype=torch.uint8), t(64, dtype=torch.uint8), (4, 6), torch.float32)
+    with fw.dual_level():
+        dual = lambda *shape: fw.make_dual(t(*shape), torch.ones(*shape))
+        for call in (lambda: act8.pack(dual(4, 6)), lambda: act8.wgrad(dual(4, 5), ck), lambda: act8.linear(dual(4, 6), t(5, 6)),
+                     lambda: act8.linear(t(4, 6), dual(5, 6)), lambda: act8.linear(t(4, 6), t(5, 6), dual(5)),
+                     lambda: act8._LinearFn.backward(None, dual(4, 5))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

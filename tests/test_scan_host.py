@@ -174,3 +174,27 @@ def test_step_takes_an_out_beside_the_state_in_the_same_rows(no_gpu):
         scan.gated_scan_step(t(1, 2), t(1, 2), buf[None, :2], out=one)
     with pytest.raises(ValueError, match="overlaps"):
         scan.gated_scan_step(t(1, 2), t(1, 2), buf.as_strided((1, 2), (0, 1), 0), out=one)
+
+
+def test_forward_mode_is_refused(no_gpu):
+    """A dual tensor has no requires_grad and its primal's pointer: without a refusal its tangent is dropped."""
+    from torch.autograd import forward_ad as fw
+    with fw.dual_level():
+        dual = lambda *shape: fw.make_dual(t(*shape), torch.ones(*shape))
+        for args in ((dual(2, 5, 3), t(2, 5, 3)), (t(2, 5, 1), dual(2, 5, 3)), (t(2, 5, 3), t(2, 5, 3), dual(2, 3))):
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    scan.gated_scan(*args)
+        for args in ((dual(4, 3), t(4, 3), t(4, 3)), (t(4, 1), dual(4, 3), t(4, 3)), (t(4, 3), t(4, 3), dual(4, 3)), (t(4, 3), t(4, 3), t(4, 3), dual(4, 3))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                scan.gated_scan_step(*args[:3], **(dict(out=args[3]) if len(args) > 3 else {}))
+
+        class Ctx:
+            pass
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            scan._ScanFn.backward(Ctx(), dual(2, 5, 3), None)
+        assert not no_gpu
+        scan.gated_scan_step(t(4, 3), t(4, 3), t(4, 3))          # (tensors without a tangent are served inside a level too)
+        assert no_gpu
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: scan.gated_scan(t(2, 5, 3), x)[0], (t(2, 5, 3),), (t(2, 5, 3),))
