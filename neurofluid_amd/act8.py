@@ -17,6 +17,7 @@ from ._lib import check, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX = 1 << 30
+_INT_MAX = (1 << 31) - 1            # what the C entries take (ctypes would keep a larger number's low 32 bits)
 
 
 def _matrix(t):
@@ -52,6 +53,8 @@ class Act8:
     def _whole(self, what):
         """The kernels read what the shape says: refuse less."""
         codes, scales = self.codes, self.scales
+        if self.rows > _MAX or self.shape[-1] > _MAX:
+            raise ValueError(f"{what}: more than {_MAX} rows or features")
         sizes = _sizes(self.rows, self.shape[-1])
         if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.numel() < sizes[0] or scales.numel() < sizes[1] or \
                 not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
@@ -125,6 +128,8 @@ def wgrad_jobs(dy, ckpt, jobs):
         raise ValueError(f"act8.wgrad: a job's numbers pass {_MAX}")
     if dy.dim() < 1 or dy.shape[-1] < 1 or ckpt.features < 1 or dy.numel() // dy.shape[-1] != ckpt.rows:
         raise ValueError(f"act8.wgrad: dy {tuple(dy.shape)} does not fit activations {ckpt.shape}")
+    if dy.shape[-1] > _MAX:
+        raise ValueError(f"act8.wgrad: more than {_MAX} columns of dy")
     if not 1 <= len(jobs) <= 16:
         raise ValueError("act8.wgrad: 1 to 16 jobs")
     ops._require_cuda(dy)
@@ -217,6 +222,8 @@ def linear(x, weight, bias=None):
     if x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.numel() == 0 or (bias is not None and bias.shape[0] != weight.shape[0]):
         raise ValueError(f"act8.linear: x {tuple(x.shape)}, weight {tuple(weight.shape)}"
                          + (f", bias {tuple(bias.shape)}" if bias is not None else "") + " do not fit")
+    if max(x.numel() // x.shape[-1], *weight.shape) > _INT_MAX:
+        raise ValueError(f"act8.linear: more than {_INT_MAX} rows or features")
     if any(t is not None and t.device != x.device for t in (weight, bias)):
         raise ValueError("act8.linear: x, weight and bias are on different devices")
     ops._require_cuda(x)

@@ -122,3 +122,19 @@ def test_forward_mode_is_refused(monkeypatch):
                      lambda: act8._LinearFn.backward(None, dual(4, 5))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_sizes_that_the_c_entries_would_cut_are_refused(monkeypatch):
+    """(Storage that is never touched: no memory behind it.)"""
+    monkeypatch.setattr(act8.ops, "_require_cuda", lambda *a: None)
+    rows = 2 ** 32 + 5
+    big = act8.Act8(torch.empty(32 * rows, dtype=torch.uint8, device="meta"), torch.empty(rows + 64, dtype=torch.uint8, device="meta"), (rows, 1), torch.float32)
+    with pytest.raises(ValueError, match="more than"):
+        big.unpack()
+    with pytest.raises(ValueError, match="more than"):
+        act8.wgrad(torch.empty(1, 1, device="meta").expand(rows, 4), big)
+    with pytest.raises(ValueError, match="more than"):
+        act8.wgrad_jobs(t(1, 1).expand(4, rows), fake(4, 6), [(0, 5, 0, 6, True)])
+    for x, w in ((t(1, 1).expand(rows, 1), t(3, 1)), (t(1, 1), t(1, 1).expand(rows, 1)), (t(1, 1).expand(1, rows), t(1, 1).expand(2, rows))):
+        with pytest.raises(ValueError, match="more than"):
+            act8.linear(x, w)
