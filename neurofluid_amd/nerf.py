@@ -220,6 +220,8 @@ class NeRF(nn.Module):
     kept in 8 bits (act8): 3.1 KB a row (masks included) instead of 10.8 KB.  Outputs and dL/dx are the fp32 path's (heads summed in another
     order: equal to the last bits); the weight gradients are those of the rounded activations.  For the default feature row (198 + 54 features)."""
 
+    act_checkpoint = None            # (modules pickled before there was a choice have none of their own)
+
     def __init__(self, D=8, W=256, in_channels_xyz=63, in_channels_dir=27, skips=(4,), act_checkpoint=None):
         super().__init__()
         if act_checkpoint not in (None, "e4m3"):

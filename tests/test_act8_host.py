@@ -138,3 +138,12 @@ def test_sizes_that_the_c_entries_would_cut_are_refused(monkeypatch):
     for x, w in ((t(1, 1).expand(rows, 1), t(3, 1)), (t(1, 1), t(1, 1).expand(rows, 1)), (t(1, 1).expand(1, rows), t(1, 1).expand(2, rows))):
         with pytest.raises(ValueError, match="more than"):
             act8.linear(x, w)
+
+
+def test_a_nerf_without_the_choice_has_none():
+    """A module that was pickled whole before act_checkpoint existed."""
+    from neurofluid_amd.nerf import NeRF
+    net = NeRF(in_channels_xyz=198, in_channels_dir=54)
+    old = NeRF.__new__(NeRF)
+    old.__setstate__({k: v for k, v in net.__dict__.items() if k != "act_checkpoint"})
+    assert old.act_checkpoint is None and "act_checkpoint" not in old.__dict__
