@@ -588,8 +588,8 @@ int nf_trans_step(const nf_trans_step_t* s /*[host]*/, const float* pos, const f
  * nf_scan_fwd writes every state (h, the storage type) and the final ones (h_last, fp32); nf_scan_bwd the gradients
  *     dx_t = g_t + u_{t+1},  u_t = A_t dx_t,  dgate_t = dx_t h_{t-1} (log_gate: u_t h_{t-1}; shared: summed over the channels),  dh0 = u_first
  * with u behind the last step = g_last.  States, products and sums are fp32; what is stored in 16 bits is rounded once, to nearest.
- * The stretch products carry states over long distances: gates are meant to be decays (|A| <= 1), larger ones overflow there sooner than
- * step by step.  Results repeat bit for bit.
+ * The stretch products carry states over long distances: gates are meant to be decays (|A| <= 1).  A product that passes the range of fp32
+ * makes a state that is not zero infinite sooner than step by step (a zero state stays zero).  Results repeat bit for bit.
  * Fill the sizes, types, strides (elements; channels are adjacent) and inputs, call nf_scan_plan (vec, cg, mode; *state_floats = the size
  * of `states`, which the forward fills if it is given and the backward needs), then allocate workspace_bytes =
  * nf_scan_workspace_bytes(s, backward) bytes, 8-byte aligned, for this call alone.  T <= 2^30, D <= 2^20, step strides < 2^18 elements (a tile's rows span less than 2^32 bytes).  h, dgate, dx are contiguous.  The backward takes the forward's plan, gate, x,

@@ -206,6 +206,17 @@ template <int TPT> __device__ __forceinline__ NfMarks nf_scan_marks(const int* s
     return m;
 }
 
+// What a zero state adds to a stretch is nothing, however large its product of gates has become (H is what the stretch gives from zero).
+__device__ __forceinline__ float nf_carry(float P, float c, float H) { return fmaf(c == 0.f ? 0.f : P, c, H); }
+// A product of gates: behind a gate of zero nothing of the entering state is left, also where the other factor has overflowed.  (Gates that are not
+// finite themselves show in H.)  The instruction is a product with 0 times anything = 0.
+__device__ __forceinline__ float nf_gates(float p, float q)
+{
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(p), "v"(q));
+    return r;
+}
+
 // (P, H) of a stretch: N products (1: one gate for all channels), VEC states.
 template <int VEC, int N, bool PACKED> struct NfAgg {
     float P[N], H[VEC];
@@ -215,15 +226,15 @@ template <int VEC, int N, bool PACKED> struct NfAgg {
     {
         if (shut()) return;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) H[k] = fmaf(P[N == 1 ? 0 : k], p.H[k], H[k]);
+        for (int k = 0; k < VEC; ++k) H[k] = nf_carry(P[N == 1 ? 0 : k], p.H[k], H[k]);
 #pragma unroll
-        for (int k = 0; k < N; ++k) P[k] *= p.P[k];
+        for (int k = 0; k < N; ++k) P[k] = nf_gates(P[k], p.P[k]);
         if (PACKED) closed = p.closed;
     }
     __device__ __forceinline__ void apply(float (&c)[VEC]) const
     {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) c[k] = shut() ? H[k] : fmaf(P[N == 1 ? 0 : k], c[k], H[k]);
+        for (int k = 0; k < VEC; ++k) c[k] = shut() ? H[k] : nf_carry(P[N == 1 ? 0 : k], c[k], H[k]);
     }
     __device__ __forceinline__ void one()
     {
@@ -580,7 +591,7 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW, M
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) me.H[k] = fmaf(A[i][N == 1 ? 0 : k], me.H[k], x.at(i, k));
 #pragma unroll
-                for (int k = 0; k < N; ++k) me.P[k] *= A[i][k];
+                for (int k = 0; k < N; ++k) me.P[k] = i == 0 ? A[i][k] : nf_gates(me.P[k], A[i][k]);
             }
         }
         nf_wave_scan<CG, 0>(me, tot, tg);
@@ -723,7 +734,7 @@ __global__ void __launch_bounds__(MODE == NF_SCAN_WAVE ? NF_SCAN_WG : 64 * NW) k
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) rv.H[k] = A[i][N == 1 ? 0 : k] * (rv.H[k] + y.at(i, k));
 #pragma unroll
-                for (int k = 0; k < N; ++k) rv.P[k] *= A[i][k];
+                for (int k = 0; k < N; ++k) rv.P[k] = i == TPT - 1 ? A[i][k] : nf_gates(rv.P[k], A[i][k]);
             }
             // forwards: the stretch as c -> P c + H, started anew where a sequence begins
             fw.one();

@@ -168,8 +168,9 @@ def gated_scan(gate, x, h0=None, *, log_gate=False, reverse=False, row_splits=No
     row_splits[s] : row_splits[s + 1] are sequence s, h0 and h_last are (n_seq, D); an empty sequence hands its h0 through, and h is zero on
     rows that belong to no sequence.
 
-    Sums, states and the carries between stretches are float32; h is rounded once.  Gates are meant to be decays, |A| <= 1: products of larger ones over long
-    stretches overflow, and where a product of gates has reached zero an infinite state goes on as NaN.  Differentiable once, in reverse mode, in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
+    Sums, states and the carries between stretches are float32; h is rounded once.  Gates are meant to be decays, |A| <= 1.  States are carried over long
+    stretches by the product of the gates: where that passes float32's range, a state that is not zero goes on as infinite even if step by step it would
+    not; where it has reached zero, an infinite state goes on as NaN.  Differentiable once, in reverse mode, in gate, x and h0; the backward reads gate and x again (they are kept), not h."""
     what = "gated_scan"
     _check(gate, x, what)
     packed = row_splits is not None

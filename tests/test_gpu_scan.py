@@ -554,3 +554,69 @@ def test_step_into_the_columns_beside_the_state(dev):
         rest = torch.ones(width, dtype=torch.bool)
         rest[second:second + D] = False
         assert torch.equal(buf.cpu()[:, rest], base[:, rest])
+
+
+def plan_of(B, T, D, dtype, gate32=False, shared=False, packed=False):
+    """Mode (0 a wave a chain, 1 chained tiles, 2 a workgroup a chain) and tiles a chain of contiguous tensors of these sizes."""
+    import ctypes
+    from neurofluid_amd import _lib
+    gs = 1 if shared else D
+    s = _lib.Scan(dtype=[F32, BF16, F16].index(dtype), gate32=int(gate32), shared=int(shared), B=B, T=T, D=D, x_sb=T * D, x_st=D, gate_sb=T * gs, gate_st=gs,
+                  row_splits=8 if packed else None)
+    n = ctypes.c_size_t()
+    assert _lib.load().nf_scan_plan(ctypes.byref(s), ctypes.byref(n)) == 0
+    return s.mode, n.value // (B * D)
+
+
+def growing(T, D, shared, reverse, gen):
+    """Gates of magnitude 2 whose products pass fp32's range many times over, in a sequence whose states and gradients do not: in processing order a gate of
+    zero in the first, middle and last third, x in the 20 steps in front of the last two of them and in the last 20, gradients in the first 20 steps
+    behind the first and the middle one."""
+    gate = torch.where(torch.rand(T, 1 if shared else D, generator=gen) < 0.5, 2.0, -2.0)
+    x, g = torch.zeros(T, D), torch.zeros(T, D)
+    cuts = [0, T // 2 + 3, T - 25]
+    gate[cuts] = 0.0
+    for a, b in ((cuts[1] - 20, cuts[1]), (cuts[2] - 20, cuts[2]), (T - 20, T)):
+        x[a:b] = torch.randn(b - a, D, generator=gen)
+    for a in cuts[:2]:
+        g[a:a + 20] = torch.randn(20, D, generator=gen)
+    return [q.flip(0) if reverse else q for q in (gate, x, g)]
+
+
+@pytest.mark.parametrize("B, T, D, dtype, mode", [(4100, 400, 4, F32, 0), (2, 700, 16, BF16, 1), (1, 9001, 64, BF16, 1), (1, 20003, 34, F32, 1), (8, 1030, 1024, BF16, 2)])
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_products_of_gates_that_overflow(dev, B, T, D, dtype, mode, shared, reverse):
+    """A zero state stays zero under gates above 1, and behind a gate of zero nothing is left, whatever the products of the stretches have become."""
+    from neurofluid_amd import scan
+    assert plan_of(B, T, D, dtype, shared=shared)[0] == mode
+    gen = torch.Generator().manual_seed(T + D)
+    ones = [growing(T, D, shared, reverse, gen) for _ in range(2)]
+    gate, x, gy = (torch.stack([ones[b % 2][k] for b in range(2)]).to(dtype) for k in range(3))
+    idx = torch.arange(B) % 2
+    h0 = torch.randn(B, D, generator=gen)
+    gd, xd, hd = gate.to(dev)[idx].requires_grad_(), x.to(dev)[idx].requires_grad_(), h0.to(dev).requires_grad_()
+    h, last = scan.gated_scan(gd, xd, hd, reverse=reverse)
+    gr = torch.autograd.grad([h, last], [gd, xd, hd], [gy.to(dev)[idx], torch.zeros_like(last)])
+    for b in sorted({0, min(1, B - 1), B - 1}):
+        w = oracle(gate[b % 2].double(), x[b % 2].double(), h0[b].double(), gy[b % 2].double(), torch.zeros(D).double(), False, reverse)
+        for name, got, dt in (("h", h, dtype), ("last", last, F32), ("dgate", gr[0], dtype), ("dx", gr[1], dtype), ("dh0", gr[2], F32)):
+            check(name, got[b], *w[name], dt)
+
+
+def test_products_that_overflow_in_packed_rows(dev):
+    from neurofluid_amd import scan
+    gen = torch.Generator().manual_seed(7)
+    lens, D = [700, 0, 3000, 90, 5000], 40
+    rs = splits_of(lens)
+    parts = [growing(n, D, False, False, gen) if n else [torch.zeros(0, D)] * 3 for n in lens]
+    gate, x, gy = (torch.cat([p[k] for p in parts]) for k in range(3))
+    h0 = torch.randn(len(lens), D, generator=gen)
+    ins = [q.to(dev).requires_grad_() for q in (gate, x, h0)]
+    h, last = scan.gated_scan(*ins, row_splits=rs.to(dev))
+    gr = torch.autograd.grad([h, last], ins, [gy.to(dev), torch.zeros_like(last)])
+    for s, n in enumerate(lens):
+        a, b = int(rs[s]), int(rs[s + 1])
+        w = oracle(gate[a:b].double(), x[a:b].double(), h0[s].double(), gy[a:b].double(), torch.zeros(D).double(), False, False)
+        for name, got in (("h", h[a:b]), ("last", last[s]), ("dgate", gr[0][a:b]), ("dx", gr[1][a:b]), ("dh0", gr[2][s])):
+            check(name, got, *w[name], F32)
