@@ -620,3 +620,44 @@ def test_products_that_overflow_in_packed_rows(dev):
         w = oracle(gate[a:b].double(), x[a:b].double(), h0[s].double(), gy[a:b].double(), torch.zeros(D).double(), False, False)
         for name, got in (("h", h[a:b]), ("last", last[s]), ("dgate", gr[0][a:b]), ("dx", gr[1][a:b]), ("dh0", gr[2][s])):
             check(name, got, *w[name], F32)
+
+
+@pytest.mark.parametrize("B, T, D, dtype, gate_kind, reverse, mode, tiles", [
+    (1, 66000, 64, BF16, "full", False, 1, 258), (1, 66000, 64, F16, "shared", True, 1, 258),        # a second set of 256 tiles
+    (1, 131500, 9, F32, "full", True, 1, 514), (1, 131500, 9, BF16, "shared", False, 1, 514),         # a third
+    (8, 1030, 1024, BF16, "full", False, 2, 5), (8, 1030, 1024, F16, "shared", True, 2, 5), (9, 1100, 1030, F32, "full", False, 2, 5),
+    (8, 1030, 1024, BF16, "full32", True, 2, 5)])
+def test_many_tiles(dev, B, T, D, dtype, gate_kind, reverse, mode, tiles):
+    """Groups of 16 tiles and sets of 16 groups, and the states that sets hand on; workgroups that walk over several tiles.  Both passes."""
+    assert plan_of(B, T, D, dtype, gate32=gate_kind == "full32", shared=gate_kind == "shared") == (mode, tiles)
+    run_dense(dev, B, T, D, dtype, gate_kind, bool(T & 1) or reverse, reverse, True, seed=T + D)
+
+
+INTO_GROUPS = ([2500, 0, 7, 900, 1, 64, 1500, 300], 11, 21)                                      # sequences over, into and inside groups
+INTO_SETS = ([30000, 0, 5, 700, 1, 20000, 256, 300, 0, 3000, 13000, 17, 1200, 2], 90, 268)        # ... and sets: one crosses row 65 536, three begin behind it
+
+
+@pytest.mark.parametrize("lens, tail, tiles, dtype, gate_kind, reverse", [
+    INTO_GROUPS + (F32, "shared", False), INTO_GROUPS + (F32, "shared", True), INTO_GROUPS + (BF16, "full", False), INTO_GROUPS + (BF16, "full", True),
+    INTO_SETS + (F32, "shared", True), INTO_SETS + (BF16, "full", False)])
+def test_packed_over_many_tiles(dev, lens, tail, tiles, dtype, gate_kind, reverse):
+    from neurofluid_amd import scan
+    D, rs = 9, splits_of(lens)
+    N, S = int(rs[-1]) + tail, len(lens)
+    assert plan_of(1, N, D, dtype, shared=gate_kind == "shared", packed=True) == (1, tiles)
+    gate, x, gy, gen = make((N, D), (N, 1 if gate_kind == "shared" else D), dtype, dtype, reverse, N + D)
+    h0, gl = torch.randn(S, D, generator=gen), torch.randn(S, D, generator=gen)
+    ins = [q.to(dev).requires_grad_() for q in (gate, x, h0)]
+    h, last = scan.gated_scan(*ins, log_gate=reverse, reverse=reverse, row_splits=rs.to(dev))
+    gr = torch.autograd.grad([h, last], ins, [gy.to(dev), gl.to(dev)])
+    h, last, gr = h.detach().cpu(), last.detach().cpu(), [q.cpu() for q in gr]
+    for s in range(S):
+        a, b = int(rs[s]), int(rs[s + 1])
+        w = oracle(gate[a:b].double(), x[a:b].double(), h0[s].double(), gy[a:b].double(), gl[s].double(), reverse, reverse)
+        check("h", h[a:b], *w["h"], dtype)
+        check("last", last[s], *w["last"], F32)
+        check("dgate", gr[0][a:b], *w["dgate"], dtype)
+        check("dx", gr[1][a:b], *w["dx"], dtype)
+        check("dh0", gr[2][s], *w["dh0"], F32)
+    for q in (h, gr[0], gr[1]):
+        assert (q[int(rs[-1]):] == 0).all()
