@@ -562,14 +562,16 @@ static int a8_jobs_ok(const char* who, int rows, int dy_cols, int x_cols, int nj
     if (njobs < 1 || njobs > A8_MAX_JOBS || !jobs) bad = "1 to 16 jobs";
     else if (rows < 0 || rows > A8_MAX || dy_cols < 1 || dy_cols > A8_MAX || x_cols < 1 || x_cols > A8_MAX) bad = "bad sizes";
     else {
-        long long outputs = 0;
+        long long outputs = 0, tiles = 0;
         for (int i = 0; i < njobs; ++i) {
             const nf_act8_job_t& j = jobs[i];
             if (j.M < 1 || j.K < 1 || j.dy_col < 0 || j.x_col < 0 || j.dy_col > dy_cols - j.M || j.x_col > x_cols - j.K) bad = "a job leaves its operands";
             else if (j.x_col % 32) bad = "a job's first feature must begin a block of 32";
+            else tiles += ((long long)j.M + 127) / 128 * (((long long)j.K + 127) / 128);          // (of the smaller kind)
             outputs += j.M;
         }
         if (!bad && outputs > A8_MAX) bad = "the jobs have too many outputs";
+        if (!bad && tiles > 0x7fffffffLL) bad = "too many tiles";
     }
     if (bad) { nf_set_error("%s: %s", who, bad); return NF_EINVAL; }
     return NF_OK;

@@ -147,3 +147,20 @@ def test_a_nerf_without_the_choice_has_none():
     old = NeRF.__new__(NeRF)
     old.__setstate__({k: v for k, v in net.__dict__.items() if k != "act_checkpoint"})
     assert old.act_checkpoint is None and "act_checkpoint" not in old.__dict__
+
+
+def test_more_tiles_than_an_int_counts():
+    """2^46 tiles, whose count in 32 bits is 0 (and was divided by): in a process of its own."""
+    import os
+    import subprocess
+    import sys
+    from neurofluid_amd import build
+    build.build()
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = "\n".join(["from neurofluid_amd import _lib", "lib = _lib.load()",
+                      "for m, k in ((30, 30), (24, 30), (30, 23)):",
+                      "    j = (_lib.Act8Job * 1)(_lib.Act8Job(0, 1 << m, 0, 1 << k, 1))",
+                      "    assert lib.nf_act8_wgrad_workspace_floats(1, 1 << m, 1 << k, 1, j) == 0",
+                      "    assert lib.nf_act8_wgrad(1, None, 1 << m, 1 << m, None, None, 1 << k, 1, 1, j, None, None, None, None) < 0 and b'tiles' in lib.nf_last_error()"])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=root)
+    assert r.returncode == 0, (r.returncode, r.stderr[-500:])
