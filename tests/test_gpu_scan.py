@@ -661,3 +661,71 @@ def test_packed_over_many_tiles(dev, lens, tail, tiles, dtype, gate_kind, revers
         check("dh0", gr[2][s], *w["dh0"], F32)
     for q in (h, gr[0], gr[1]):
         assert (q[int(rs[-1]):] == 0).all()
+
+
+@pytest.mark.parametrize("B, T, D, dtype, reverse", [(3, 203, 96, BF16, False), (2, 77, 31, F16, True), (1, 3001, 200, BF16, True)])
+def test_one_gate_a_step_in_32_bits_beside_16_bit_rows(dev, B, T, D, dtype, reverse):
+    from neurofluid_amd import scan
+    gate, x, gy, gen = make((B, T, D), (B, T, 1), dtype, F32, True, T + D)
+    h0, gl = torch.randn(B, D, generator=gen), torch.randn(B, D, generator=gen)
+    ins = [q.to(dev).requires_grad_() for q in (gate, x, h0)]
+    h, last = scan.gated_scan(*ins, log_gate=True, reverse=reverse)
+    gr = torch.autograd.grad([h, last], ins, [gy.to(dev), gl.to(dev)])
+    assert h.dtype == dtype and [q.dtype for q in gr] == [F32, dtype, F32]
+    for b in range(B):
+        w = oracle(gate[b].double(), x[b].double(), h0[b].double(), gy[b].double(), gl[b].double(), True, reverse)
+        for name, got, dt in (("h", h, dtype), ("last", last, F32), ("dgate", gr[0], F32), ("dx", gr[1], dtype), ("dh0", gr[2], F32)):
+            check(name, got[b], *w[name], dt)
+
+
+def test_packed_rows_in_a_graph(dev):
+    """Captured forward and backward of packed rows, replayed over other splits, values and eager work of their own."""
+    from neurofluid_amd import scan
+    gate, x, gy, gen = make((6000, 40), (6000, 40), BF16, BF16, False, 15)
+    cuts = [torch.tensor(c, device=dev) for c in ([0, 100, 100, 5000, 6000], [7, 8, 3000, 3000, 5990], [0, 0, 0, 6000, 6000], [5, 2000, 4000, 4001, 4002])]
+    xs = [(x * k).to(dev) for k in (1, 2, 3, 4)]
+    g0, y0, h0 = gate.to(dev), gy.to(dev), torch.randn(4, 40, generator=gen).to(dev)
+
+    def both(rs, xx):
+        ins = [q.detach().requires_grad_() for q in (g0, xx, h0)]
+        h, last = scan.gated_scan(*ins, row_splits=rs)
+        return (h.detach(), last.detach()) + torch.autograd.grad([h, last], ins, [y0, torch.ones_like(last)])
+    rs, xx = cuts[0].clone(), xs[0].clone()
+    both(rs, xx)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(rs, xx)
+    for it in range(6):
+        rs.copy_(cuts[it % 4])
+        xx.copy_(xs[(it + 1) % 4])
+        graph.replay()
+        want = both(cuts[it % 4], xs[(it + 1) % 4])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), it
+
+
+@pytest.mark.parametrize("B, T, D, mode", [(1, 4_200_000, 520, 1), (33, 65536, 1024, 2), (2_200_000, 16, 64, 0)])
+def test_gradients_past_32_bit_offsets(dev, B, T, D, mode):
+    """Both passes over more than 2^31 elements.  The gradients that enter are zero but for the last rows of the last batch, and gates of
+    1/2 forget: there the results are those of the same rows on their own, and in front of them no gradient is left."""
+    from neurofluid_amd import scan
+    assert B * T * D > 2 ** 31 and plan_of(B, T, D, BF16, shared=True)[0] == mode
+    n = min(T, 300)
+    x = torch.zeros(B, T, D, dtype=BF16, device=dev)
+    x[-1, T - n:].normal_()
+    g = torch.zeros_like(x)
+    g[-1, T - n + n // 2:].normal_()
+    gate = torch.full((B, T, 1), 0.5, dtype=BF16, device=dev).requires_grad_()
+    x.requires_grad_()
+    h, last = scan.gated_scan(gate, x)
+    dgate, dx = torch.autograd.grad(h, [gate, x], g)
+    tail = x[-1, T - n:].detach().cpu().double()
+    w = oracle(torch.full((n, 1), 0.5).double(), tail, torch.zeros(D).double(), g[-1, T - n:].cpu().double(), torch.zeros(D).double(), False, False)
+    check("h", h[-1, T - n:], *w["h"], BF16)
+    check("last", last[-1], *w["last"], F32)
+    check("dx", dx[-1, T - n:], *w["dx"], BF16)
+    check("dgate", dgate[-1, T - n:], *w["dgate"], BF16)
+    assert not h[-1, :T - n].any() and not dx[-1, :max(T - 1000, 0)].any() and not dgate[-1, :T - n].any()
+    if B > 1:
+        assert not h[:-1].any() and not dx[:-1].any() and not last[:-1].any()
