@@ -2,8 +2,9 @@
 
 What torch autograd keeps for the linear layers of models/nerf.py:55-81 are their inputs, in 32 bits.  ``pack`` keeps them as e4m3 codes with one
 power-of-two scale for every 32 features of a row (1.03 bytes a value, off by at most 2^-4 of itself), ``wgrad`` computes dW = dy^T x^ and
-db = sum dy from the codes as they are, ``linear`` is the layer that does both, and ``NeRF(..., act_checkpoint="e4m3")`` trains on it.
-Forward values and the gradients of the inputs are those of the exact activations; only the weights' gradients see the 8 bits.
+db = sum dy from the codes as they are, ``linear`` is the layer that does both, and the module ``NeRF(..., act_checkpoint="e4m3")`` trains on it.
+Forward values and the gradients of the inputs are those of the exact activations; only the weights' gradients see the 8 bits.  Codes, what is
+unpacked from them and ``wgrad``'s results carry no gradients of their own.
 There is no torch fallback: CPU tensors raise.
 """
 import ctypes

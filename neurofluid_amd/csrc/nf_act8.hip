@@ -217,13 +217,17 @@ extern "C" int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* sc
 //
 // Tile: (64 C) x (64 C) outputs a workgroup, each of 4 waves a quarter, 32 rows a slab, two slabs in LDS: while one is multiplied the next is
 // packed into the other and the one after that is on its way in registers; one barrier a slab.  C = 4 (256 x 256: 64 matrix instructions a
-// slab and plane for 32 fragment reads) where that fills the chip, else C = 2 (two workgroups a CU).  The rows are split into slices, whose
-// partial tiles a second launch adds in a fixed order.
+// slab and plane for 32 fragment reads) from 32 such tiles on, else C = 2 (two workgroups a CU).  C = 4 against 2, us a call with the second launch, bf16:
+// 32 768 rows, 64 tiles 270 / 400, 32 tiles 155 / 207, 16 tiles 99 / 122, 8 tiles 65 / 73; 6001 rows, 32 tiles 54 / 56, 16 tiles 45 / 45; 63 001 rows, one
+// tile 43 / 36.  (fp32: 633 / 832, 339 / 432, 202 / 242, 125 / 139; 94 / 94, 68 / 60; 62 / 52.  For many rows the border could lie lower.)  The
+// rows are split into slices, whose partial tiles a second launch adds in a fixed order.
 //
 // What bounds it: 32 768 rows, 2 048 x 2 048, bf16: 294 us = 935 TFLOP/s (the library's 8192^3 bf16 product reaches 1 093), the matrix unit busy 47 % of
 // the cycles at the clock that its power leaves, 28 % of a wave's cycles waiting (fragments out of LDS: 96 KB a slab and workgroup).
 // 63 001 rows, 256 x 256, fp32 (three planes): 48 us for 81 MB of operands (each read by two tiles) and 24.8 GFLOP in bf16.  Neither bound is
 // near (16 us, 23 us): 124 slices of four tiles leave a workgroup 16 slabs, of which the first and the last three run unoverlapped.
+// By dy's type, us a call with the second launch: 63 001 rows 256 x 256 fp32 52, fp16 64, bf16 45; 32 768 rows 2 048 x 2 048 fp32 703, fp16 1 155,
+// bf16 319.  fp16 with its two planes takes longer than fp32 with three; why is not known.
 // ------------------------------------------------------------------------------------------------
 #define A8_MAX_JOBS 16
 #define A8_SLAB 32

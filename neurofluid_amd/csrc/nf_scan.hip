@@ -28,10 +28,19 @@ static int scan_vec(const void* p, int64_t sb, int64_t st, int size)
     return v;
 }
 
-// Lanes: as many channels a block as D has, a cache line's 64 of 16 bits or 32 of 32 bits at the most (65 536 steps x 256 channels in fp32: 46 us
-// forward with 32, 52 with 64; in fp16 43 with 64, 45 with 32).  Modes: thousands of chains, or chains of few steps, take a wave each; from 8 192 channels on a
-// workgroup each (2048 steps, fp16, forward / backward: 16 384 channels 40 / 76 us against 59 / 92 chained, 8 192 29 / 46 against 31 / 46,
-// 4 096 and 4096 steps 47 / 77 against 33 / 46); fewer ones are chained.
+// Figures: forward / backward, us, as timed with this plan and with others forced.
+// Lanes: as many channels a block as D has, a cache line's 64 of 16 bits or 32 of 32 bits at the most (65 536 steps x 256 channels, fp32:
+// 47 / 69 with 32, 58 / 77 with 64; fp16 46 / 65 with 64, 45 / 69 with 32).  Fewer channels, 40 000 x 192 fp32, one gate a step: four channels a lane,
+// D = 4 65 / 94 with one lane (four 77 / 107, eight 117 / 193), 16 199 / 288 with four (eight 219 / 304, one 283 / 448).  One or two channels a
+// lane (rows that are not aligned for more), lanes across: D = 1 42 / 58 with two (eight 43 / 85, 32 130 / 315), 3 52 / 105 with eight (two 101 / 196,
+// 32 126 / 359); 32 of them pay from many channels on: D = 34 (two a lane) 532 / 746 against 669 / 904 with eight, but 18 374 / 589 against
+// 320 / 443 and 9 (one a lane) 240 / 429 against 230 / 307: between 8 and 16 groups eight lanes would be the better choice.
+// Modes: thousands of chains, or chains of few steps, take a wave each; from 8 192 channels on a workgroup each (2048 steps, bf16: 16 384
+// channels 40 / 72 against 47 / 87 chained and 176 / 291 by waves, 8 192 32 / 53 against 33 / 54; 4 096 channels and 4096 steps 51 / 90 against
+// 36 / 55); fewer ones are chained.  From 4 096 chains on by waves: 4 096 x 192 x 32 fp32 35 / 50 against 41 / 100 by workgroups, though
+// 4 096 x 1024 x 32 226 / 344 against 204 / 312.  Chains of one or two tiles gain nothing from being chained, and a tile that they do not
+// fill costs more than waves: 64 x 400 x 64 fp32 14 / 17 against 8 / 12 by workgroups, 700 x 192 x 32 13 / 25 by workgroups against 12 / 18
+// by waves, 2000 x 600 x 1 27 / 41 against 12 / 16.
 extern "C" int nf_scan_plan(nf_scan_t* s, size_t* state_floats)
 {
     const int rc = scan_check(s, __func__);

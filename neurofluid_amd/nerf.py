@@ -217,7 +217,9 @@ class NeRF(nn.Module):
     fp32-MFMA kernels.
 
     act_checkpoint="e4m3" (not in the reference): what a training forward keeps for the weight gradients — the activations and the feature row — is
-    kept in 8 bits (act8): 3.1 KB a row (masks included) instead of 10.8 KB.  Outputs and dL/dx are the fp32 path's (heads summed in another
+    kept in 8 bits (act8): 3.1 KB a row (masks included) instead of 10.8 KB.  Within one call the fp32 activations are there whole until they are
+    packed, so the forward's own peak is 14.1 KB a row instead of 10.9: what falls is what several calls, or other layers, hold until the
+    backward.  It is this module's own forward that does so; RenderNet's fused passes keep fp32 whatever its networks say.  Outputs and dL/dx are the fp32 path's (heads summed in another
     order: equal to the last bits); the weight gradients are those of the rounded activations.  For the default feature row (198 + 54 features)."""
 
     act_checkpoint = None            # (modules pickled before there was a choice have none of their own)
