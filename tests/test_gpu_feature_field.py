@@ -197,3 +197,35 @@ def test_feature_field_along_rays(dev):
         bound = notes[2 - i][1]                    # (the backward met the layers from the last to the first)
         assert ((grads[1 + i].cpu().double() - want[1 + i]).abs() <= bound).all(), i
         assert rel(grads[4 + i], want[4 + i]) <= 1e-4
+
+
+def test_what_is_saved_may_leave_the_gpu_in_between(dev):
+    """Saved tensors that autograd's hooks keep in host memory, and passes that are run again for the backward, give the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    from neurofluid_amd import act8, scan
+    g = torch.Generator().manual_seed(31)
+    x, w, b = torch.randn(600, 20, generator=g), torch.randn(16, 20, generator=g), torch.randn(16, generator=g)
+    h0, rs = torch.randn(3, 16, generator=g), torch.tensor([0, 250, 250, 590])
+    lg = -torch.rand(600, 17, generator=g)[:, 1:]              # (rows of 17: read one by one)
+
+    def run(how):
+        ins = [q.to(dev).requires_grad_() for q in (x, w, b, h0)]
+        gate = torch.empty(600, 17, device=dev)[:, 1:].copy_(lg).detach().requires_grad_()
+
+        def f(x, w, b, h0, gate):
+            y = act8.linear(x, w, b)
+            h, last = scan.gated_scan(gate, y, h0, log_gate=True, row_splits=rs.to(dev))
+            z, _ = scan.gated_scan(gate.view(1, 600, 16) if gate.is_contiguous() else gate[None], h[None], log_gate=True, reverse=True)
+            return z.square().sum() + last.square().sum()
+        if how == "host":
+            with torch.autograd.graph.save_on_cpu():
+                loss = f(*ins, gate)
+        elif how == "again":
+            loss = checkpoint(f, *ins, gate, use_reentrant=False)
+        else:
+            loss = f(*ins, gate)
+        return torch.autograd.grad(loss, ins + [gate])
+    want = run("")
+    assert all(q.abs().sum() > 0 for q in want)
+    for how in ("host", "again"):
+        assert all(torch.equal(a, b) for a, b in zip(run(how), want)), how
