@@ -210,13 +210,9 @@ template <int TPT> __device__ __forceinline__ NfMarks nf_scan_marks(const int* s
 // What a zero state adds to a stretch is nothing, however large its product of gates has become (H is what the stretch gives from zero).
 __device__ __forceinline__ float nf_carry(float P, float c, float H) { return fmaf(c == 0.f ? 0.f : P, c, H); }
 // A product of gates: behind a gate of zero nothing of the entering state is left, also where the other factor has overflowed.  (Gates that are not
-// finite themselves show in H.)  The instruction is a product with 0 times anything = 0.
-__device__ __forceinline__ float nf_gates(float p, float q)
-{
-    float r;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(p), "v"(q));
-    return r;
-}
+// finite themselves show in H.)  v_mul_legacy_f32: 0 times anything = 0.  As LLVM's intrinsic, not as inline assembly: its result goes to row
+// exchanges and comes from exp, and the compiler sets the wait states between those and an instruction only where it knows what that is.
+extern "C" __device__ __attribute__((const)) float nf_gates(float p, float q) __asm("llvm.amdgcn.fmul.legacy");
 
 // (P, H) of a stretch: N products (1: one gate for all channels), VEC states.
 template <int VEC, int N, bool PACKED> struct NfAgg {
