@@ -635,7 +635,8 @@ int nf_act8_unpack(int dtype, const uint8_t* codes, const uint8_t* scales, int r
  *     dW_j[m][k] = sum_r dy[r][dy_col_j + m] x^[r][x_col_j + k],     db_j[m] = sum_r dy[r][dy_col_j + m]    (bias_j != 0)
  * x^ = the values the codes stand for.  fp32 results: every product is exact (but for what of dy lies below 2^-133), sums are
  * fp32 in a fixed order.  dweights holds the dW_j [M][K] one
- * behind the other, dbias the db_j of the jobs that ask for one.  x_col_j must be a multiple of 32.  rows = 0 gives zeros.
+ * behind the other, dbias the db_j of the jobs that ask for one.  x_col_j must be a multiple of 32.  At most 2^31 - 1 tiles of
+ * 128 x 128 outputs over all jobs.  rows = 0 gives zeros.
  * workspace: nf_act8_wgrad_workspace_floats floats. */
 typedef struct { int dy_col, M, x_col, K, bias; } nf_act8_job_t;
 size_t nf_act8_wgrad_workspace_floats(int rows, int dy_cols, int x_cols, int njobs, const nf_act8_job_t* jobs /*[host]*/);

@@ -27,12 +27,12 @@
 //
 // What bounds them: a step costs two or three products for each value read, so memory does wherever the arithmetic keeps up.  A pass reads and
 // writes every tensor once (bytes below, over the time; a large copy on the same card moves 5.2 TB/s).
-//   walk: 8 x 2048 x 2048 bf16, fp32 gates, 268 MB forward 53 us (5.1 TB/s), 470 MB backward 91 us (5.2 TB/s);
+//   walk: 8 x 2048 x 2048 bf16, fp32 gates, 268 MB forward 52 us (5.2 TB/s), 470 MB backward 88 us (5.3 TB/s);
 //   wave: 4096 x 192 x 32 fp32, 205 MB forward 33 us (6.3 TB/s: part of it comes from the last-level cache), 309 MB backward 48 us;
-//     256 x 512 x 1024 fp16, 805 MB forward 160 us (5.0 TB/s), 1.3 GB backward 294 us (4.6 TB/s);
-//     40 000 x 192 x 4 fp32, 277 MB 60 us (4.6 TB/s): four channels a lane share a gate, so exp and the exchange across 64 lanes weigh on
-//     few values, and waves wait for their turn to issue (60 % of their cycles) more than for memory (26 %);
-//   chain: 4 x 4096 x 1024 bf16, 101 MB forward 29 us (3.5 TB/s); 65 537 x 256 fp16, 101 MB forward 39 us (2.6 TB/s), 168 MB backward 58 us (2.9 TB/s):
+//     256 x 512 x 1024 fp16, 805 MB forward 161 us (5.0 TB/s), 1.3 GB backward 291 us (4.6 TB/s);
+//     40 000 x 192 x 4 fp32, 277 MB 59 us (4.7 TB/s): four channels a lane share a gate, so exp and the exchange across 64 lanes weigh on
+//     few values, and waves wait for their turn to issue (61 % of their cycles) more than for memory (26 %);
+//   chain: 4 x 4096 x 1024 bf16, 101 MB forward 30 us (3.4 TB/s); 65 537 x 256 fp16, 101 MB forward 40 us (2.5 TB/s), 168 MB backward 58 us (2.9 TB/s):
 //     a tile's entry reaches the others through memory, group by group and set by set, and a workgroup has no loads under way while it waits for
 //     them (a wave waits 74 % of its cycles).
 #pragma once
